@@ -1,0 +1,422 @@
+"""Cases of the paged 8-bit KV cache: appending to it with the position rotation on the way, and attention over it.
+
+``op`` names the call:
+
+* ``append``: new keys and values of a batch of sequences into their pages, keys and queries turned to their positions
+  (and into the rotated basis) on the way; the pages written are read back as the values that they stand for;
+* ``attend``: causal attention of each sequence's newest tokens over its pages;
+* ``step``: the two as a layer makes them for a batch, the new tokens appended and attended to.
+
+Pages hold 8-bit codes and one power-of-two scale for each page and head: keys ``[pages, heads, page_size, dim]``,
+values ``[pages, heads, dim, page_size]``.  A page table row lists a sequence's pages; lengths count the new tokens.
+"""
+
+from __future__ import annotations
+
+import math
+import random
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+BYTES = {"f32": 4, "f16": 2, "bf16": 2}
+LEAST_SCALE = 2.0**-40
+
+
+def listed():
+    return [
+        # one decoded token of a chat: latency and launches; its page is half full
+        dict(name="append_token", op="append", seqs=1, new=1, past=480, kv=8, group=4, dim=128, page=64, dtype="f16", rotary=128, axes=1, basis=True),
+        # one decoded token of each sequence of a served batch, small pages
+        dict(name="append_batch", op="append", seqs=64, new=1, past=4000, kv=4, group=4, dim=256, page=16, dtype="bf16", rotary=64, axes=1, basis=True),
+        # ragged prompts in float32, positions turned in part of the dimensions, no rotated basis
+        dict(name="append_ragged_f32", op="append", seqs=5, new=640, past=300, kv=4, group=2, dim=64, page=32, dtype="f32", rotary=32, axes=1, basis=False),
+        # an image and its text: positions of three axes (time, height, width)
+        dict(name="append_image", op="append", seqs=1, new=2601, past=77, kv=4, group=8, dim=128, page=32, dtype="bf16", rotary=128, axes=3, basis=True),
+        # a long prompt: the rate of the whole pass
+        dict(name="append_prompt", op="append", seqs=1, new=32768, past=0, kv=8, group=4, dim=128, page=64, dtype="f16", rotary=128, axes=1, basis=True),
+        # the first tokens of a chat on a model without grouped queries: latency
+        dict(name="attend_short", op="attend", seqs=1, new=1, past=511, kv=8, group=1, dim=128, page=64, dtype="f16"),
+        # one sequence at the benchmark's context and heads
+        dict(name="attend_32k", op="attend", seqs=1, new=1, past=32767, kv=8, group=4, dim=128, page=64, dtype="f16"),
+        # float32 queries at the widest head and a long context
+        dict(name="attend_128k_f32", op="attend", seqs=1, new=1, past=131071, kv=2, group=4, dim=256, page=64, dtype="f32"),
+        # a served batch of very different lengths, small pages, eight query heads to a head of the cache
+        dict(name="attend_batch", op="attend", seqs=48, new=1, past=6000, kv=4, group=8, dim=128, page=16, dtype="bf16"),
+        # a few drafted tokens of each sequence at once
+        dict(name="attend_drafts", op="attend", seqs=8, new=5, past=9000, kv=8, group=4, dim=64, page=32, dtype="f16"),
+        # a chunk of a long prompt: products, not memory
+        dict(name="attend_chunk", op="attend", seqs=1, new=2000, past=6001, kv=4, group=4, dim=256, page=64, dtype="bf16"),
+        # one layer's step of a served batch, both calls
+        dict(name="step_batch", op="step", seqs=24, new=1, past=3000, kv=4, group=4, dim=256, page=64, dtype="bf16", rotary=64, axes=1, basis=True),
+    ]
+
+
+# What a drawn call has at most, near what the largest listed ones have:
+MOST_PAIRS = 2.0e8  # query rows times keys, all heads
+MOST_CACHED = 6.0e7  # elements of the keys in the cache
+MOST_NEW = 6.0e8  # bytes of new queries, keys and values, read and written
+
+
+def _log_uniform(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["append", "append", "attend", "attend", "attend", "step"])
+    c = dict(op=op, kv=rng.choice([1, 2, 3, 4, 8]), group=rng.choice([1, 2, 3, 4, 5, 6, 7, 8]), dim=rng.choice([64, 128, 256]),
+             page=rng.choice([16, 32, 64]), dtype=rng.choice(["f16", "bf16", "bf16", "f32"]))
+    c["seqs"] = rng.choice([1, 1, _log_uniform(rng, 2, 64)])
+    c["new"] = rng.choice([1, 1, rng.randint(2, 16), _log_uniform(rng, 17, 8192)])
+    c["past"] = rng.choice([0, _log_uniform(rng, 1, 131072), _log_uniform(rng, 1, 16384)])
+    heads = c["kv"] * c["dim"] * c["seqs"]
+    c["new"] = max(1, min(c["new"], int(MOST_NEW / heads / (2 + 2 * c["group"]) / BYTES[c["dtype"]])))
+    c["past"] = max(0, min(c["past"], int(MOST_CACHED / heads)))
+    if op != "append":
+        rows = c["seqs"] * c["kv"] * c["group"]
+        c["new"] = max(1, min(c["new"], int(math.sqrt(MOST_PAIRS / rows))))
+        c["past"] = max(0, min(c["past"], int(MOST_PAIRS / rows / c["new"])))
+    if op != "attend":
+        c["rotary"] = rng.choice([0, c["dim"] // 4, c["dim"] // 2, c["dim"]])
+        c["axes"] = rng.choice([1, 1, 2, 3]) if c["rotary"] else 1
+        c["basis"] = rng.random() < 0.7
+    return c
+
+
+# ------------------------------------------------------------------ inputs
+
+
+def _lengths(case):
+    """New tokens and total length of each sequence; a batch is ragged, and now and then one of them has nothing."""
+    rng = random.Random(f"{case['seqs']} {case['past']} {case['new']}")
+    if case["seqs"] == 1:
+        return [case["new"]], [case["past"] + case["new"]]
+    new = [case["new"] if case["new"] <= 16 else rng.randint(1, case["new"]) for _ in range(case["seqs"])]
+    past = [int(case["past"] * 2.0 ** rng.uniform(-2, 0.5)) for _ in range(case["seqs"])]
+    if case["op"] == "attend" and case["seqs"] > 8 and case["new"] == 1:
+        past[rng.randrange(case["seqs"])] = -1  # a slot of the batch without a sequence: length zero
+    return new, [p + n for p, n in zip(past, new)]
+
+
+def _pair_axes(case):
+    """The axis whose position turns each pair of dimensions: a contiguous section of the pairs for each."""
+    pairs, axes = case["rotary"] // 2, case["axes"]
+    return tuple(min(i * axes // pairs, axes - 1) for i in range(pairs))
+
+
+def _randn(g, shape, dtype=torch.float32):
+    return torch.randn(shape, generator=g, device="cuda", dtype=torch.float32).to(dtype)
+
+
+def _scale_of(largest):
+    """The least power of two, 2^-40 or more, of which `largest` is at most 127."""
+    m, e = torch.frexp(largest)
+    return torch.ldexp(torch.ones_like(largest), e - 7 + (m > 127.0 / 128.0).to(e.dtype)).clamp_min(LEAST_SCALE)
+
+
+def _filled_pages(g, count, case, transposed, spread):
+    """Pages of normal rows, held as codes and scales."""
+    rows = _randn(g, (count, case["kv"], case["page"], case["dim"]))
+    if spread:
+        rows *= torch.exp(0.3 * _randn(g, (1, case["kv"], 1, case["dim"])) + 0.2 * _randn(g, (count, case["kv"], case["page"], 1)))
+    scales = _scale_of(rows.abs().amax((2, 3)))
+    codes = torch.round(rows / scales[:, :, None, None]).to(torch.int8)
+    return (codes.transpose(2, 3) if transposed else codes).contiguous(), scales
+
+
+def _inputs(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    new, total = _lengths(case)
+    page, dim, kv, heads, dtype = case["page"], case["dim"], case["kv"], case["kv"] * case["group"], TYPES[case["dtype"]]
+    width = max(1, max(-(-t // page) for t in total))
+    used = [max(0, -(-t // page)) for t in total]
+    count = sum(used) + 3
+    order = torch.randperm(count, generator=g, device="cuda", dtype=torch.int64).to(torch.int32)
+    table = torch.full((len(new), width), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for b, n in enumerate(used):
+        table[b, :n] = order[at : at + n]
+        at += n
+    s = dict(case=case, table=table, lens=torch.tensor([max(0, t) for t in total], dtype=torch.int32, device="cuda"), starts=None)
+    tokens = sum(new)
+    if max(new) > 1:
+        s["starts"] = torch.tensor([sum(new[:b]) for b in range(len(new) + 1)], dtype=torch.int32, device="cuda")
+    s["most"] = max(new)
+    s["key_pages"], s["key_scales"] = _filled_pages(g, count, case, False, True)
+    s["value_pages"], s["value_scales"] = _filled_pages(g, count, case, True, False)
+    s["query"] = _randn(g, (tokens, heads, dim), dtype)
+    if case["op"] == "attend":
+        return s
+    s["key"] = (_randn(g, (tokens, kv, dim)) * torch.exp(0.5 * _randn(g, (1, kv, dim)))).to(dtype)
+    s["value"] = _randn(g, (tokens, kv, dim), dtype)
+    s["cos"] = s["sin"] = s["positions"] = s["pair_axes"] = s["left"] = s["right"] = None
+    if case["rotary"]:
+        inv = 1.0 / 10000.0 ** (torch.arange(0, case["rotary"], 2, device="cuda", dtype=torch.float64) / case["rotary"])
+        angle = torch.arange(max(total) + 1, device="cuda", dtype=torch.float64)[:, None] * inv[None]
+        angle = torch.cat([angle, angle], dim=-1)
+        s["cos"], s["sin"] = angle.cos().float(), angle.sin().float()
+        if case["axes"] > 1:  # time, height and width of a patch, each below the sequence's length
+            s["positions"] = (torch.rand((case["axes"], tokens), generator=g, device="cuda") * max(total)).to(torch.int32)
+            s["pair_axes"] = _pair_axes(case)
+            s["axis"] = torch.tensor(s["pair_axes"] * 2, device="cuda")
+    if case["basis"]:
+        s["left"], s["right"] = (torch.where(_randn(g, (dim,)) < 0, -1.0, 1.0) for _ in range(2))
+    first = [(t - n) // page for n, t in zip(new, total)]
+    last = [(t - 1) // page for t in total]
+    s["touched"] = torch.cat([table[b, first[b] : last[b] + 1] for b in range(len(new))])
+    return s
+
+
+def prepare(case, seed):
+    return _inputs(case, seed)
+
+
+# ------------------------------------------------------------------ the plain forms
+
+
+def _rows(s):
+    """Sequence, and position in it, of each new token."""
+    lens = s["lens"].long()
+    if s["starts"] is None:
+        seq = torch.arange(lens.numel(), device="cuda")
+        return seq, lens - 1
+    starts = s["starts"].long()
+    n = starts[1:] - starts[:-1]
+    seq = torch.repeat_interleave(torch.arange(lens.numel(), device="cuda"), n, output_size=s["query"].shape[0])
+    return seq, lens[seq] - n[seq] + torch.arange(s["query"].shape[0], device="cuda") - starts[seq]
+
+
+def _turned(x, s, positions):
+    """Rotary positions on the first dimensions of [tokens, heads, dim] rows, halves paired."""
+    if s["cos"] is None:
+        return x
+    r = s["cos"].shape[1]
+    if s["positions"] is None:
+        cos, sin = s["cos"][positions], s["sin"][positions]
+    else:
+        row = s["positions"].long()[s["axis"]].t()  # [tokens, r]
+        col = torch.arange(r, device=x.device)
+        cos, sin = s["cos"][row, col], s["sin"][row, col]
+    a = x[..., :r]
+    half = torch.cat((-a[..., r // 2 :], a[..., : r // 2]), dim=-1)
+    return torch.cat((a * cos[:, None] + half * sin[:, None], x[..., r:]), dim=-1)
+
+
+def _butterflies(x, step):
+    if step == x.shape[-1]:
+        return x
+    y = x.reshape(*x.shape[:-1], -1, 2, step)
+    y = torch.stack((y[..., 0, :] + y[..., 1, :], y[..., 0, :] - y[..., 1, :]), dim=-2)
+    return _butterflies(y.reshape(x.shape), 2 * step)
+
+
+def _based(x, s):
+    """Rows in the rotated basis: signs, Walsh-Hadamard transform over sqrt(dim), signs."""
+    if s["left"] is None:
+        return x
+    root = torch.full((1,), math.sqrt(x.shape[-1]), device=x.device, dtype=x.dtype)
+    return _butterflies(x * s["right"], 1) / root * s["left"]
+
+
+def _append_stream(rows, pages, scales, ids, table, seq, pos):
+    """Rows [tokens, heads, dim] into pages [pages, heads, page, dim] (`ids`: those written), their scales grown and
+    old codes held anew."""
+    page = pages.shape[2]
+    at, slot = table[seq, pos // page].long(), pos % page
+    finite = torch.where(torch.isfinite(rows), rows.abs(), 0.0).amax(-1)
+    largest = torch.zeros_like(scales).index_reduce_(0, at, finite, "amax")
+    first = torch.full((pages.shape[0],), page, device=rows.device).index_reduce_(0, at, slot, "amin")  # slots kept
+    mine = (first < page)[:, None]
+    fresh = _scale_of(largest)
+    grown = torch.where(first[:, None] == 0, fresh, torch.maximum(scales, fresh))
+    kept = torch.arange(page, device=rows.device)[None, :] < first[:, None]
+    old = pages[ids]  # only the pages written
+    ratio = (scales[ids] / grown[ids])[:, :, None, None]
+    pages[ids] = torch.where(kept[ids][:, None, :, None], torch.round(old.float() * ratio).to(torch.int8), old)
+    scales.copy_(torch.where(mine, grown, scales))
+    codes = torch.nan_to_num(rows / scales[at][:, :, None], nan=0.0).clamp(-127, 127)
+    pages[at, :, slot] = torch.round(codes).to(torch.int8)
+
+
+def _append(s):
+    seq, pos = _rows(s)
+    ids = s["touched"].long()
+    key = _based(_turned(s["key"].float(), s, pos), s)
+    _append_stream(key, s["key_pages"], s["key_scales"], ids, s["table"], seq, pos)
+    values = s["value_pages"].transpose(2, 3)  # a view: rows go to the transposed pages
+    _append_stream(s["value"].float(), values, s["value_scales"], ids, s["table"], seq, pos)
+    return _based(_turned(s["query"].float(), s, pos), s).to(s["query"].dtype)
+
+
+def _read_back(s):
+    at = s["touched"].long()
+    k = s["key_pages"][at].float() * s["key_scales"][at][:, :, None, None]
+    v = s["value_pages"][at].float() * s["value_scales"][at][:, :, None, None]
+    return k.to(torch.bfloat16), v.transpose(2, 3).to(torch.bfloat16)  # 7 bits and a power of two: bfloat16 holds them
+
+
+def _attend(s, query, wide=torch.float32):
+    page, dim, group = s["key_pages"].shape[2], query.shape[-1], s["case"]["group"]
+    kv, batch, width, most = s["key_pages"].shape[1], s["table"].shape[0], s["table"].shape[1], s["most"]
+    at = s["table"].long().clamp_min(0)
+    k = (s["key_pages"][at].to(wide) * s["key_scales"][at][..., None, None]).transpose(1, 2).reshape(batch, kv, width * page, dim)
+    v = (s["value_pages"][at].to(wide) * s["value_scales"][at][..., None, None]).permute(0, 2, 1, 4, 3).reshape(batch, kv, width * page, dim)
+    seq, pos = _rows(s)
+    lane = torch.arange(query.shape[0], device=query.device) - (seq if s["starts"] is None else s["starts"].long()[seq])
+    q = torch.zeros(batch, most, kv * group, dim, dtype=wide, device=query.device)
+    q[seq, lane] = query.to(wide)
+    q = q.reshape(batch, most, kv, group, dim).transpose(1, 2).reshape(batch, kv, most * group, dim)
+    last = torch.full((batch, most), -1, dtype=torch.int64, device=query.device)
+    last[seq, lane] = pos
+    seen = torch.arange(width * page, device=query.device) <= last.repeat_interleave(group, 1)[:, None, :, None]
+    score = torch.matmul(q, k.transpose(2, 3).contiguous()).mul_(1.0 / math.sqrt(dim)).masked_fill_(~seen, -math.inf)
+    top = score.amax(-1, keepdim=True)
+    weight = score.sub_(torch.where(torch.isinf(top), 0.0, top)).exp_()
+    total = weight.sum(-1, keepdim=True)
+    out = torch.matmul(weight, v) / torch.where(total == 0, 1.0, total)
+    out = out.reshape(batch, kv, most, group, dim).transpose(1, 2).reshape(batch, most, kv * group, dim)
+    return out[seq, lane]
+
+
+def run(s):
+    op = s["case"]["op"]
+    if own:
+        return _own(s, op)
+    if op == "attend":
+        return _attend(s, s["query"]).to(s["query"].dtype)
+    query = _append(s)
+    if op == "append":
+        return (query, *_read_back(s))
+    return (_attend(s, query).to(query.dtype), *_read_back(s))
+
+
+# ------------------------------------------------------------------ the framework's calls
+
+
+def _own(s, op):
+    package = str(Path(__file__).resolve().parents[1] / "torque-mlx_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    from torque_hip import ops
+
+    pool = {n: s[n] for n in ("key_pages", "value_pages", "key_scales", "value_scales")}
+    batch = dict(page_table=s["table"], context_lens=s["lens"], token_starts=s["starts"])
+    query = s["query"]
+    if op != "attend":
+        query = ops.paged_append(s["key"], s["value"], query=query, cos=s["cos"], sin=s["sin"], positions=s["positions"],
+                                 pair_axes=s["pair_axes"], signs_left=s["left"], signs_right=s["right"], **pool, **batch)
+    if op == "append":
+        return (query, *ops.paged_dequantize(s["touched"], dtype=torch.bfloat16, **pool))
+    out = ops.paged_attention(query, max_tokens=s["most"], **pool, **batch)
+    if op == "attend":
+        return out
+    return (out, *ops.paged_dequantize(s["touched"], dtype=torch.bfloat16, **pool))
+
+
+# ------------------------------------------------------------------ what a pass cannot do without
+
+
+def work(case):
+    new, total = _lengths(case)
+    size, kv, dim, page = BYTES[case["dtype"]], case["kv"], case["dim"], case["page"]
+    heads, tokens = kv * case["group"], sum(new)
+    moved = flops = 0.0
+    if case["op"] != "attend":
+        moved += tokens * dim * (2 * kv * (size + 1) + heads * size * (2 if case["op"] == "append" else 1))
+        moved += 8.0 * tokens * case["rotary"] + (4.0 * case["axes"] * tokens if case["axes"] > 1 else 0)
+        flops += tokens * dim * ((kv + heads) * (math.log2(dim) + 2 if case["basis"] else 3) + 4 * kv)
+        pages = sum((t - 1) // page - (t - n) // page + 1 for n, t in zip(new, total))
+        moved += 2 * pages * kv * page * dim * (1 + 2)  # read back
+    if case["op"] != "append":
+        keys = sum(max(0, t) for t in total)
+        moved += 2 * keys * kv * (dim + 4 / page) + tokens * heads * dim * size * (2 if case["op"] == "attend" else 1)
+        flops += 4.0 * heads * dim * sum(n * t - n * (n - 1) / 2 for n, t in zip(new, total) if t > 0)
+    return {"bytes": moved, "flops": flops}
+
+
+# ------------------------------------------------------------------ the same in 64 bits
+
+
+def _hadamard(dim, device):
+    bits = torch.arange(dim, device=device)
+    both = bits[:, None] & bits[None, :]
+    odd = sum((both >> k) & 1 for k in range(8)) % 2
+    return torch.where(odd == 1, -1.0, 1.0).double() / math.sqrt(dim)
+
+
+def _exact_turned(x, s, b, n, total, start):
+    """Rows of one sequence, turned pair by pair as complex numbers, then into the rotated basis."""
+    x = x.double()
+    if s["cos"] is not None:
+        r = s["cos"].shape[1]
+        turn = torch.complex(s["cos"].double(), s["sin"].double())[:, : r // 2]
+        if s["positions"] is None:
+            turn = turn[total - n : total]
+        else:
+            turn = torch.stack([turn[s["positions"][a, start : start + n].long(), i] for i, a in enumerate(s["pair_axes"])], dim=-1)
+        z = torch.complex(x[..., : r // 2].contiguous(), x[..., r // 2 : r].contiguous()) * turn[:, None]
+        x = torch.cat((z.real, z.imag, x[..., r:]), dim=-1)
+    if s["left"] is not None:
+        x = torch.matmul(x * s["right"].double(), _hadamard(x.shape[-1], x.device)) * s["left"].double()
+    return x
+
+
+def _exact_pages(pages, scales, ids, rows, c):
+    """One sequence's pages in 64 bits, page by page: values [touched, heads, page, dim]; codes and scales are put back."""
+    page, n = pages.shape[2], rows.shape[0]
+    done = 0
+    for j, p in enumerate(ids):
+        kept = c % page if j == 0 else 0
+        take = min(page - kept, n - done)
+        x = rows[done : done + take].transpose(0, 1)  # [heads, take, dim]
+        top = x.abs().amax((1, 2))
+        fresh = torch.exp2(torch.ceil(torch.log2(top.clamp_min(1e-300) / 127.0))).clamp_min(LEAST_SCALE)
+        s = fresh if kept == 0 else torch.maximum(scales[p].double(), fresh)
+        old = torch.round(pages[p].double() * (scales[p].double() / s)[:, None, None])
+        pages[p, :, :kept] = old[:, :kept].to(torch.int8)
+        pages[p, :, kept : kept + take] = torch.round(x / s[:, None, None]).clamp(-127, 127).to(torch.int8)
+        scales[p] = s.float()
+        done += take
+
+
+def exact(case, seed):
+    s = _inputs(case, seed)
+    new, total = _lengths(case)
+    op, group, kv, page, dim = case["op"], case["group"], case["kv"], case["page"], case["dim"]
+    if op == "append" and sum(new) > 70000 or sum(-(-n // page) for n in new) > 6000:
+        return None
+    query, out, start = [], [], 0
+    table = s["table"].tolist()
+    kp, vp = s["key_pages"], s["value_pages"].transpose(2, 3)
+    for b, (n, t) in enumerate(zip(new, total)):
+        q = s["query"][start : start + n].double()
+        if op != "attend":
+            q = _exact_turned(s["query"][start : start + n], s, b, n, t, start)
+            ids = table[b][(t - n) // page : (t - 1) // page + 1]
+            _exact_pages(kp, s["key_scales"], ids, _exact_turned(s["key"][start : start + n], s, b, n, t, start), t - n)
+            _exact_pages(vp, s["value_scales"], ids, s["value"][start : start + n].double(), t - n)
+        query.append(q)
+        start += n
+        if op == "append":
+            continue
+        o = torch.zeros(n, kv * group, dim, dtype=torch.float64, device="cuda")
+        ids = table[b][: -(-t // page)] if t > 0 else []
+        for h in range(kv if ids else 0):
+            k = (kp[ids, h].double() * s["key_scales"][ids, h].double()[:, None, None]).reshape(-1, dim)[:t]
+            v = (vp[ids, h].double() * s["value_scales"][ids, h].double()[:, None, None]).reshape(-1, dim)[:t]
+            hidden = torch.arange(t, device="cuda")[None] > torch.arange(t - n, t, device="cuda")[:, None]
+            for j in range(h * group, (h + 1) * group):
+                w = torch.matmul(q[:, j].contiguous(), k.t().contiguous()) / math.sqrt(dim)
+                o[:, j] = torch.matmul(torch.softmax(w.masked_fill(hidden, -math.inf), dim=-1), v)
+        out.append(o)
+    if op == "attend":
+        return torch.cat(out)
+    at = s["touched"].long()
+    k = kp[at].double() * s["key_scales"][at].double()[:, :, None, None]
+    v = vp[at].double() * s["value_scales"][at].double()[:, :, None, None]
+    return (torch.cat(query) if op == "append" else torch.cat(out), k, v)
