@@ -115,7 +115,8 @@ def _randn(g, shape, dtype=torch.float32):
 def _scale_of(largest):
     """The least power of two, 2^-40 or more, of which `largest` is at most 127."""
     m, e = torch.frexp(largest)
-    return torch.ldexp(torch.ones_like(largest), e - 7 + (m > 127.0 / 128.0).to(e.dtype)).clamp_min(LEAST_SCALE)
+    scale = torch.ldexp(torch.ones_like(largest), e - 7 + (m > 127.0 / 128.0).to(e.dtype))
+    return torch.where(largest > 0, scale, 0.0).clamp_min(LEAST_SCALE)
 
 
 def _filled_pages(g, count, case, transposed, spread):
