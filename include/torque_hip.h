@@ -42,7 +42,7 @@ enum {
   TQ_ERR_LAUNCH = -3       /* HIP launch failure (Python: RuntimeError) */
 };
 
-enum { TQ_F32 = 0, TQ_F16 = 1, TQ_BF16 = 2 /* tq_rotary and tq_unrotate_gate only */ };
+enum { TQ_F32 = 0, TQ_F16 = 1, TQ_BF16 = 2 /* tq_rotary, tq_unrotate_gate and the paged cache only */ };
 
 /* tq_append / tq_quantize_dequantize flags (reference cache_mlx.py:52-54) */
 enum { TQ_ROTATE_KEYS = 1, TQ_ROTATE_VALUES = 2 };
@@ -352,6 +352,82 @@ int tq_unrotate_gate(const float* attn, int heads, int64_t tokens, int head_dim,
  * NULL) are bound to the kernel as in tq_decode_timed. */
 int tq_stream_read(const void* data, size_t bytes, float* sink, int n_blocks, hipStream_t stream, hipEvent_t start,
                    hipEvent_t stop);
+
+/* ---- Paged 8-bit KV cache (no reference counterpart: the reference's caches
+ * hold one sequence in one slab of 2/3/4-bit codes).
+ *
+ * Pages of T = page_size slots (16, 32 or 64), head_dim D (64, 128, 256):
+ *   key_pages    int8  [num_pages, kv_heads, T, D]
+ *   value_pages  int8  [num_pages, kv_heads, D, T]   (transposed)
+ *   key_scales, value_scales  float32 [num_pages, kv_heads], positive
+ * A held value is code * scale; codes are -127..127 and appends write scales
+ * that are powers of two, 2^-40 or more.  Pages are 16-byte aligned.
+ *
+ * A batch: page_table int32 [batch, max_pages] (rows table_stride apart) lists
+ * each sequence's pages; context_lens int32 [batch] counts its tokens, those of
+ * the call included; token_starts int32 [batch + 1], not decreasing, gives the
+ * rows [starts[b], starts[b+1]) of the call that are sequence b's newest tokens
+ * (NULL: one row each).  They lie on the device and are not read by the host.
+ * Page numbers outside [0, num_pages) and places outside the table are passed
+ * over: such tokens are not written, and not seen.
+ *
+ * Rows [tokens, heads, D] have unit stride along D; other strides are in
+ * elements.  dtypes: TQ_F32, TQ_F16 or TQ_BF16. */
+
+enum { TQ_TABLES_BY_TOKEN = 32 }; /* tq_paged_append flag: row i of the tables belongs to row i of the call */
+
+/* Appends keys and values to the pages.  Keys (and queries, into query_out
+ * [tokens, query_heads, D], when query is not NULL) are turned by rotary
+ * positions on the way: y[d] = x[d] cos[r, d] + rotate_half(x)[d] sin[r, d] for
+ * d < rotary_dim (0: none), r the cache position, or positions[tokens] (int32,
+ * or int64 with positions_wide), or the row itself (TQ_TABLES_BY_TOKEN).  With
+ * axes 2 to 4, positions is [axes, tokens] (rows positions_stride apart) and
+ * pair_axes (host, rotary_dim / 2 bytes) names the axis that turns each pair
+ * (d, d + rotary_dim / 2).  A key whose r is outside [0, table_rows) is not
+ * written, a query becomes NaN.  Then, with signs, keys and queries go into the
+ * rotated basis as tq_append takes them there (values with TQ_ROTATE_VALUES).
+ *
+ * A page's scale is the least power of two by which the largest finite element
+ * is at most 127; it never shrinks while a sequence's earlier tokens are in the
+ * page, and where it grows their codes are rounded anew.  Infinities are held as
+ * the largest code, NaN as 0.  Slots after the sequence's end keep what they
+ * held.  A page may be appended to for one sequence only in a call. */
+int tq_paged_append(const void* key, int64_t key_token_stride, int64_t key_head_stride, const void* value,
+                    int64_t value_token_stride, int64_t value_head_stride, int kv_dtype, const void* query,
+                    int64_t query_token_stride, int64_t query_head_stride, int query_dtype, int query_heads,
+                    void* query_out, int64_t tokens, int kv_heads, int head_dim, int8_t* key_pages, int8_t* value_pages,
+                    float* key_scales, float* value_scales, int num_pages, int page_size, const int32_t* page_table,
+                    int64_t table_stride, int max_pages, const int32_t* context_lens, const int32_t* token_starts,
+                    int batch, const void* cos, int64_t cos_stride, const void* sin, int64_t sin_stride, int table_dtype,
+                    int64_t table_rows, int rotary_dim, const void* positions, int positions_wide,
+                    int64_t positions_stride, int axes, const uint8_t* pair_axes, const float* signs_left,
+                    const float* signs_right, int flags, hipStream_t stream);
+
+/* The values of pages page_ids [count] (device): keys_out and values_out
+ * [count, kv_heads, T, D] of out_dtype; a number outside the pool gives zeros. */
+int tq_paged_dequantize(const int32_t* page_ids, int64_t count, const int8_t* key_pages, const int8_t* value_pages,
+                        const float* key_scales, const float* value_scales, int num_pages, int page_size, int kv_heads,
+                        int head_dim, void* keys_out, void* values_out, int out_dtype, hipStream_t stream);
+
+/* Bytes that tq_paged_attention needs for its partial sums (0: none; bad
+ * arguments give 0 too).  ragged: token_starts is not NULL; num_cus <= 0: the
+ * current device's compute units. */
+size_t tq_paged_attention_workspace_bytes(int64_t tokens, int batch, int ragged, int query_heads, int kv_heads,
+                                          int head_dim, int max_pages, int page_size, int64_t max_tokens, int num_cus);
+
+/* Causal attention of each sequence's newest tokens over its pages: row i of n
+ * stands at position context_lens[b] - n + i and sees the keys up to it;
+ * a row that sees none gives zeros.  out has the query's dtype; rows of no
+ * sequence are not written.  max_tokens: the most rows that any sequence has (a
+ * hint that only chooses the kernel; <= 0: unknown).  The workspace needs no
+ * initialisation and may be used again by calls ordered on one stream. */
+int tq_paged_attention(const void* query, int64_t query_token_stride, int64_t query_head_stride, int query_dtype,
+                       int64_t tokens, int query_heads, int kv_heads, int head_dim, const int8_t* key_pages,
+                       const int8_t* value_pages, const float* key_scales, const float* value_scales, int num_pages,
+                       int page_size, const int32_t* page_table, int64_t table_stride, int max_pages,
+                       const int32_t* context_lens, const int32_t* token_starts, int batch, int64_t max_tokens,
+                       float scale, void* workspace, size_t workspace_bytes, void* out, int64_t out_token_stride,
+                       int64_t out_head_stride, hipStream_t stream);
 
 #ifdef __cplusplus
 }

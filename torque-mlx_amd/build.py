@@ -3,8 +3,8 @@
     python torque-mlx_amd/build.py            # or __graft_entry__.build()
     python torque-mlx_amd/build.py --asan OUT.so   # host-only AddressSanitizer build
 
-Compiles csrc/torque_hip.hip with hipcc into torque_hip/libtorque_hip.so,
-in-tree.  Packed-FP32 VALU ops are disabled for all device code.  The
+Compiles csrc/torque_hip.hip and csrc/paged.hip with hipcc, side by side, and
+links them into torque_hip/libtorque_hip.so, in-tree.  Packed-FP32 VALU ops are disabled for all device code.  The
 atomic optimizer is off for device code: it rewrites a single lane's LDS
 atomic (the split kernels' tile counter) into a wave-wide form that waits
 for the result at once, where the kernels want it one iteration later.
@@ -16,11 +16,13 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 ROOT = Path(__file__).resolve().parent
 REPO = ROOT.parent
-SOURCE = ROOT / "csrc" / "torque_hip.hip"
+SOURCES = (ROOT / "csrc" / "torque_hip.hip", ROOT / "csrc" / "paged.hip")
 OUTPUT = ROOT / "torque_hip" / "libtorque_hip.so"
 ARCH = os.environ.get("TORQUE_HIP_ARCH", "gfx950")
 
@@ -29,7 +31,6 @@ HIPCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-Xclang",
     "-target-feature",
     "-Xclang",
@@ -60,14 +61,8 @@ def asan_runtime() -> Path:
     return hits[-1]
 
 
-def build_library(verbose: bool = False, asan: bool = False, output: Path | None = None) -> Path:
-    """Compile the library to `output` (default: the in-tree libtorque_hip.so; the ASan build has no
-    default location and needs one)."""
-    if asan and output is None:
-        raise ValueError("the AddressSanitizer build needs an output path outside the package")
-    out = Path(output) if output is not None else OUTPUT
-    flags = [f for f in HIPCC_FLAGS if not (asan and f == "-O3")] + (ASAN_FLAGS if asan else [])
-    cmd = [hipcc(), *flags, "-I", str(REPO / "include"), "-I", str(ROOT / "csrc"), str(SOURCE), "-o", str(out) + ".tmp"]
+def _run(cmd: list[str], verbose: bool) -> str:
+    """Run one compiler command; its messages, or RuntimeError."""
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
@@ -75,6 +70,23 @@ def build_library(verbose: bool = False, asan: bool = False, output: Path | None
     stderr = "\n".join(line for line in proc.stderr.splitlines() if noise not in line)
     if proc.returncode != 0:
         raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{stderr}")
+    return stderr
+
+
+def build_library(verbose: bool = False, asan: bool = False, output: Path | None = None) -> Path:
+    """Compile the library to `output` (default: the in-tree libtorque_hip.so; the ASan build has no
+    default location and needs one)."""
+    if asan and output is None:
+        raise ValueError("the AddressSanitizer build needs an output path outside the package")
+    out = Path(output) if output is not None else OUTPUT
+    flags = [f for f in HIPCC_FLAGS if not (asan and f == "-O3")] + (ASAN_FLAGS if asan else [])
+    with tempfile.TemporaryDirectory(prefix="torque_hip_") as tmp:
+        objects = [str(Path(tmp) / (source.stem + ".o")) for source in SOURCES]
+        compile_ = [hipcc(), *flags, "-I", str(REPO / "include"), "-I", str(ROOT / "csrc"), "-c"]
+        with ThreadPoolExecutor(len(SOURCES)) as pool:
+            done = list(pool.map(lambda so: _run([*compile_, str(so[0]), "-o", so[1]], verbose), zip(SOURCES, objects)))
+        done.append(_run([hipcc(), *flags, "-shared", *objects, "-o", str(out) + ".tmp"], verbose))
+    stderr = "\n".join(text for text in done if text.strip())
     os.replace(str(out) + ".tmp", out)
     if verbose and stderr.strip():
         print(stderr, file=sys.stderr)

@@ -9,34 +9,6 @@
 // stands for, in the same order, so the rotary output is bit-identical.
 #pragma once
 
-// Element types of the layer's tensors.
-enum { kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 2 };
-
-__device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int type) {
-  if (type == kTypeF32) return static_cast<const float*>(p)[i];
-  const uint16_t h = static_cast<const uint16_t*>(p)[i];
-  return type == kTypeF16 ? __half2float(__ushort_as_half(h)) : __uint_as_float(static_cast<uint32_t>(h) << 16);
-}
-// Bits of x rounded to nearest even in bfloat16 (a NaN stays one).
-__device__ __forceinline__ uint16_t bf16_bits(float x) {
-  const uint32_t u = __float_as_uint(x);
-  if (x != x) return static_cast<uint16_t>((u >> 16) | 0x40u);
-  return static_cast<uint16_t>((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
-__device__ __forceinline__ float round_as(float x, int type) {
-  if (type == kTypeF32) return x;
-  if (type == kTypeF16) return __half2float(__float2half(x));
-  return __uint_as_float(static_cast<uint32_t>(bf16_bits(x)) << 16);
-}
-__device__ __forceinline__ void store_as(void* p, int64_t i, float x, int type) {
-  if (type == kTypeF32)
-    static_cast<float*>(p)[i] = x;
-  else if (type == kTypeF16)
-    static_cast<__half*>(p)[i] = __float2half(x);
-  else
-    static_cast<uint16_t*>(p)[i] = bf16_bits(x);
-}
-
 // [heads, tokens, D] rows with unit stride along D.
 struct RowView {
   const void* data;

@@ -35,24 +35,35 @@
 
 #include "torque_hip.h"
 #include "tq_device.hpp"
+#include "tq_host.hpp"
 
 using namespace tq;
 
 namespace {
-
 thread_local std::string g_last_error;
+}  // namespace
 
-int fail(int code, const std::string& msg) {
+int tq::fail(int code, const std::string& msg) {
   g_last_error = msg;
   return code;
 }
 
-int launch_status(const char* what) {
+int tq::launch_status(const char* what) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(TQ_ERR_LAUNCH, std::string(what) + ": " + hipGetErrorString(e));
   g_last_error.clear();
   return TQ_OK;
 }
+
+int tq::device_cu_count() {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 256;
+  int cus = 0;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
+  return cus;
+}
+
+namespace {
 
 bool valid_bits(int b) { return b == 2 || b == 3 || b == 4; }
 bool valid_head_dim(int d) { return d == 64 || d == 128 || d == 256; }
@@ -1716,14 +1727,6 @@ int default_splits(int units, int64_t seq_len, int num_cus, int wgs_per_cu) {
   return static_cast<int>(ns);
 }
 
-int device_cu_count() {
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess) return 256;
-  int cus = 0;
-  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 256;
-  return cus;
-}
-
 // Workspace layout: [ml: Lq * ns * 2][acc: Lq * ns * D][cur_s: Lq][cur_v: Lkv * D]
 // floats, Lq = layers * query heads, Lkv = layers * KV heads, each section
 // 256-byte aligned.
@@ -2380,11 +2383,6 @@ int with_d(int head_dim, Args&&... args) {
   }
   return fail(TQ_ERR_UNSUPPORTED, "Unsupported head dimension: " + std::to_string(head_dim));
 }
-
-// Workgroups per launch of the row kernels (fwht, append, unpack, rotary,
-// gate).  A HIP launch holds at most 2^32 - 1 work-items; larger calls are cut
-// into launches of at most this many workgroups, in stream order.
-constexpr int64_t kMaxLaunchBlocks = int64_t(1) << 20;
 
 // Grid of one launch of a kernel with a wavefront per row, `rows` left to do.
 dim3 row_grid(int64_t rows) {

@@ -18,6 +18,9 @@ from torque_hip.ops import (
     decode_packed_attention_split_batched,
     decode_packed_attention_split_batched_with_current,
     metal_available,
+    paged_append,
+    paged_attention,
+    paged_dequantize,
     quantize_and_pack_rows,
     quantize_and_pack_rows_dual,
 )
@@ -74,6 +77,9 @@ __all__ = [
     "load_torque_artifact",
     "metal_available",
     "packed_words_for_head_dim",
+    "paged_append",
+    "paged_attention",
+    "paged_dequantize",
     "quantize_and_pack_rows",
     "quantize_and_pack_rows_dual",
     "run_qwen_decode_runtime_benchmark",

@@ -28,7 +28,7 @@ TQ_ERR_LAUNCH = -3
 
 TQ_F32 = 0
 TQ_F16 = 1
-TQ_BF16 = 2  # tq_rotary and tq_unrotate_gate only
+TQ_BF16 = 2  # tq_rotary, tq_unrotate_gate and the paged cache only
 
 TQ_ROTATE_KEYS = 1
 TQ_ROTATE_VALUES = 2
@@ -37,6 +37,7 @@ TQ_INVERSE_OUTPUT = 2
 TQ_F32_PRODUCTS = 4
 TQ_MATRIX_PRODUCTS = 8
 TQ_ONE_LAUNCH = 16
+TQ_TABLES_BY_TOKEN = 32
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
@@ -103,6 +104,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_p, _p, _i, _i, _i, _i64, _i, _i64, _i64, _i64, _i64, _p, _p, _i, _i64, _i64, _i, _p, _p, _i, _p],
     ),
     "tq_unrotate_gate": (_i, [_p, _i, _i64, _i, _i64, _i64, _p, _i, _i64, _i64, _p, _p, _p, _i, _p]),
+    "tq_paged_append": (
+        _i,
+        [_p, _i64, _i64, _p, _i64, _i64, _i, _p, _i64, _i64, _i, _i, _p, _i64, _i, _i, _p, _p, _p, _p, _i, _i, _p, _i64,
+         _i, _p, _p, _i, _p, _i64, _p, _i64, _i, _i64, _i, _p, _i, _i64, _i, _p, _p, _p, _i, _p],
+    ),
+    "tq_paged_dequantize": (_i, [_p, _i64, _p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _i, _p]),
+    "tq_paged_attention_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i, _i, _i, _i64, _i]),
+    "tq_paged_attention": (
+        _i,
+        [_p, _i64, _i64, _i, _i64, _i, _i, _i, _p, _p, _p, _p, _i, _i, _p, _i64, _i, _p, _p, _i, _i64, _f, _p, _sz, _p,
+         _i64, _i64, _p],
+    ),
     "tq_stream_read": (_i, [_p, _sz, _p, _i, _p, _p, _p]),
 }
 
@@ -150,7 +163,8 @@ def check(rc: int) -> None:
     raise TorqueHIPError(message or f"libtorque_hip error {rc}")
 
 
-_NOT_STATUS = {"tq_abi_version", "tq_last_error", "tq_decode_workspace_bytes", "tq_decode_split_kernel"}
+_NOT_STATUS = {"tq_abi_version", "tq_last_error", "tq_decode_workspace_bytes", "tq_decode_split_kernel",
+               "tq_paged_attention_workspace_bytes"}
 
 
 def call(name: str, *args) -> int:

@@ -18,6 +18,7 @@ from torque_hip import _lib
 from torque_hip._lib import TQ_F32, hip_available
 from torque_hip._tensors import codes_to_device, device, dtype_code, shape_of, stream_handle, to_device
 from torque_hip.layout import PackedKVLayout
+from torque_hip.paged import paged_append, paged_attention, paged_dequantize
 
 __all__ = [
     "accumulate_packed_values",
@@ -28,6 +29,9 @@ __all__ = [
     "decode_packed_attention_split_batched_with_current",
     "hip_available",
     "metal_available",
+    "paged_append",
+    "paged_attention",
+    "paged_dequantize",
     "quantize_and_pack_rows",
     "quantize_and_pack_rows_dual",
     "score_packed_query",
