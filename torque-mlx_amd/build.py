@@ -3,8 +3,8 @@
     python torque-mlx_amd/build.py            # or __graft_entry__.build()
     python torque-mlx_amd/build.py --asan OUT.so   # host-only AddressSanitizer build
 
-Compiles csrc/torque_hip.hip and csrc/paged.hip with hipcc, side by side, and
-links them into torque_hip/libtorque_hip.so, in-tree.  Packed-FP32 VALU ops are disabled for all device code.  The
+Compiles the csrc/*.hip sources with hipcc, side by side, and links them into
+torque_hip/libtorque_hip.so, in-tree.  Packed-FP32 VALU ops are disabled for all device code.  The
 atomic optimizer is off for device code: it rewrites a single lane's LDS
 atomic (the split kernels' tile counter) into a wave-wide form that waits
 for the result at once, where the kernels want it one iteration later.
@@ -22,7 +22,7 @@ from pathlib import Path
 
 ROOT = Path(__file__).resolve().parent
 REPO = ROOT.parent
-SOURCES = (ROOT / "csrc" / "torque_hip.hip", ROOT / "csrc" / "paged.hip")
+SOURCES = tuple(ROOT / "csrc" / name for name in ("torque_hip.hip", "paged_append.hip", "paged_attention.hip"))
 OUTPUT = ROOT / "torque_hip" / "libtorque_hip.so"
 ARCH = os.environ.get("TORQUE_HIP_ARCH", "gfx950")
 

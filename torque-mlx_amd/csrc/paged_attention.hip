@@ -1,0 +1,144 @@
+// paged_attention.hip -- attention over the paged 8-bit KV cache: kernels' launches
+// and C ABI.  Declarations are in include/torque_hip.h.
+//
+// Kernels
+//   paged_split_kernel   attention of few rows over long contexts
+//   paged_merge_kernel   the parts of rows whose keys were cut, as one
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "paged_attention.hpp"
+#include "paged_host.hpp"
+
+using namespace tq;
+
+namespace {
+
+// How a call's attention is cut: `items` units of R rows, `workgroups` to a KV
+// head (0: a workgroup to an item and no merge).
+struct PagedPlan {
+  int64_t items;
+  int workgroups;
+  size_t acc_bytes, ml_bytes, cut_bytes;
+};
+
+constexpr int kSplitRows = 16;
+constexpr int kLeastTiles = 8;  // tiles of 64 keys that a workgroup takes at least
+
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+PagedPlan plan_attention(int64_t tokens, int batch, bool ragged, int group, int kv_heads, int head_dim, int max_pages,
+                         int page_size, int num_cus) {
+  PagedPlan p{};
+  p.items = ragged ? tokens * group / kSplitRows + batch : static_cast<int64_t>(batch) * ((group + kSplitRows - 1) / kSplitRows);
+  const int64_t tiles = (static_cast<int64_t>(max_pages) * page_size + kTile - 1) / kTile;  // of one sequence, at most
+  const int64_t units = p.items * kv_heads;
+  if (tiles <= kLeastTiles || units >= 16 * static_cast<int64_t>(num_cus)) return p;
+  const int64_t fill = std::max<int64_t>(1, 2 * static_cast<int64_t>(num_cus) / kv_heads);
+  const int64_t most = std::max<int64_t>(1, (p.items * std::max<int64_t>(tiles, 1) + kLeastTiles - 1) / kLeastTiles);
+  p.workgroups = static_cast<int>(std::min(fill, most));
+  const size_t slots = static_cast<size_t>(p.workgroups) * kv_heads * 2 * kSplitRows;
+  p.acc_bytes = align256(slots * head_dim * sizeof(float));
+  p.ml_bytes = align256(slots * 2 * sizeof(float));
+  p.cut_bytes = align256(static_cast<size_t>(p.items) * kv_heads * sizeof(int2));
+  return p;
+}
+
+template <int D, int PLANES>
+int launch_split(const PagedAttentionArgs& a, const PagedPlan& plan, hipStream_t stream) {
+  const unsigned heads = static_cast<unsigned>(a.batch.kv_heads);
+  if (plan.workgroups == 0) {
+    hipLaunchKernelGGL((paged_split_kernel<D, PLANES, false>), dim3(static_cast<unsigned>(plan.items), heads), dim3(kBlock), 0, stream, a);
+    return launch_status("paged_split_kernel");
+  }
+  hipLaunchKernelGGL((paged_split_kernel<D, PLANES, true>), dim3(static_cast<unsigned>(plan.workgroups), heads), dim3(kBlock), 0, stream, a);
+  const int rc = launch_status("paged_split_kernel");
+  if (rc) return rc;
+  const int64_t rows = static_cast<int64_t>(a.batch.tokens) * heads * a.group;
+  hipLaunchKernelGGL((paged_merge_kernel<D, kSplitRows>), dim3(static_cast<unsigned>((rows + kWavesPerBlock - 1) / kWavesPerBlock)),
+                     dim3(kBlock), 0, stream, a);
+  return launch_status("paged_merge_kernel");
+}
+
+template <int D>
+int launch_attention_d(const PagedAttentionArgs& a, const PagedPlan& plan, hipStream_t stream) {
+  return a.query_type == TQ_F32 ? launch_split<D, 3>(a, plan, stream) : launch_split<D, 2>(a, plan, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tq_paged_attention_workspace_bytes(int64_t tokens, int batch, int ragged, int query_heads, int kv_heads,
+                                          int head_dim, int max_pages, int page_size, int64_t max_tokens, int num_cus) {
+  if (tokens <= 0 || batch <= 0 || kv_heads <= 0 || query_heads <= 0 || query_heads % kv_heads != 0 || max_pages < 0 ||
+      check_pages(1, page_size, kv_heads, head_dim) != TQ_OK)
+    return 0;
+  if (num_cus <= 0) num_cus = device_cu_count();
+  (void)max_tokens;
+  const PagedPlan p = plan_attention(tokens, batch, ragged != 0, query_heads / kv_heads, kv_heads, head_dim, max_pages, page_size, num_cus);
+  return p.acc_bytes + p.ml_bytes + p.cut_bytes;
+}
+
+int tq_paged_attention(const void* query, int64_t query_token_stride, int64_t query_head_stride, int query_dtype,
+                       int64_t tokens, int query_heads, int kv_heads, int head_dim, const int8_t* key_pages,
+                       const int8_t* value_pages, const float* key_scales, const float* value_scales, int num_pages,
+                       int page_size, const int32_t* page_table, int64_t table_stride, int max_pages,
+                       const int32_t* context_lens, const int32_t* token_starts, int batch, int64_t max_tokens,
+                       float scale, void* workspace, size_t workspace_bytes, void* out, int64_t out_token_stride,
+                       int64_t out_head_stride, hipStream_t stream) {
+  int rc = check_pages(num_pages, page_size, kv_heads, head_dim);
+  if (rc) return rc;
+  rc = check_batch(tokens, batch, max_pages, table_stride, token_starts);
+  if (rc) return rc;
+  rc = check_heads(tokens, query_heads, kv_heads);
+  if (rc) return rc;
+  if (!type_ok(query_dtype)) return fail(TQ_ERR_BAD_ARG, "dtypes must be F32, F16 or BF16");
+  if (!std::isfinite(scale)) return fail(TQ_ERR_BAD_ARG, "scale must be finite");
+  if (tokens == 0 || batch == 0) return TQ_OK;
+  if (!query || !key_pages || !value_pages || !key_scales || !value_scales || !context_lens || (max_pages > 0 && !page_table) || !out)
+    return fail(TQ_ERR_BAD_ARG, "null pointer argument");
+  if (!aligned16(key_pages) || !aligned16(value_pages)) return fail(TQ_ERR_BAD_ARG, "pages must be 16-byte aligned");
+  const int group = query_heads / kv_heads;
+  const PagedPlan plan = plan_attention(tokens, batch, token_starts != nullptr, group, kv_heads, head_dim, max_pages, page_size, device_cu_count());
+  if (plan.items > INT_MAX) return fail(TQ_ERR_BAD_ARG, "tokens x group exceeds one launch");
+  const size_t need = plan.acc_bytes + plan.ml_bytes + plan.cut_bytes;
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(TQ_ERR_BAD_ARG, "workspace too small: " + std::to_string(workspace_bytes) + " bytes, the call needs " + std::to_string(need));
+  if (need > 0 && !aligned16(workspace)) return fail(TQ_ERR_BAD_ARG, "the workspace must be 16-byte aligned");
+  PagedAttentionArgs a{};
+  a.batch = batch_of(page_table, table_stride, max_pages, context_lens, token_starts, batch, tokens, num_pages, page_size, kv_heads);
+  a.query = query;
+  a.query_type = query_dtype;
+  a.q_token_stride = query_token_stride;
+  a.q_head_stride = query_head_stride;
+  a.out = out;
+  a.o_token_stride = out_token_stride;
+  a.o_head_stride = out_head_stride;
+  a.group = group;
+  a.key_pages = key_pages;
+  a.value_pages = value_pages;
+  a.key_scales = key_scales;
+  a.value_scales = value_scales;
+  a.score_scale = scale * 1.4426950408889634f;
+  a.items = static_cast<int>(plan.items);
+  a.workgroups = plan.workgroups;
+  a.least_tiles = kLeastTiles;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  a.acc = reinterpret_cast<float*>(ws);
+  a.ml = reinterpret_cast<float*>(ws + plan.acc_bytes);
+  a.cut = reinterpret_cast<int2*>(ws + plan.acc_bytes + plan.ml_bytes);
+  switch (head_dim) {
+    case 64:
+      return launch_attention_d<64>(a, plan, stream);
+    case 128:
+      return launch_attention_d<128>(a, plan, stream);
+    default:
+      return launch_attention_d<256>(a, plan, stream);
+  }
+}
+
+}  // extern "C"

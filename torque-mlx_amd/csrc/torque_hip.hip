@@ -167,27 +167,6 @@ __device__ __forceinline__ float div_sqrt_d(float x, float sqrt_d) {
   return __fdiv_rn(x, sqrt_d);
 }
 
-// v[i] += pair * (the partner lane's v[i]) for 16 elements, one operation
-// each: the compiler leaves the DPP move and the fma apart.  The two wait
-// states in front are what a DPP read needs after a VALU write.
-template <int CTRL>
-__device__ __forceinline__ void pair_step(float (&v)[16], float pair) {
-#define TQ_PAIR(i, mode) "v_fmac_f32_dpp %" #i ", %" #i ", %16 " mode " row_mask:0xf bank_mask:0xf\n\t"
-#define TQ_PAIRS(mode)                                                                                             \
-  asm("s_nop 1\n\t" TQ_PAIR(0, mode) TQ_PAIR(1, mode) TQ_PAIR(2, mode) TQ_PAIR(3, mode) TQ_PAIR(4, mode)           \
-          TQ_PAIR(5, mode) TQ_PAIR(6, mode) TQ_PAIR(7, mode) TQ_PAIR(8, mode) TQ_PAIR(9, mode) TQ_PAIR(10, mode)   \
-              TQ_PAIR(11, mode) TQ_PAIR(12, mode) TQ_PAIR(13, mode) TQ_PAIR(14, mode) TQ_PAIR(15, mode)            \
-      : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7]),            \
-        "+v"(v[8]), "+v"(v[9]), "+v"(v[10]), "+v"(v[11]), "+v"(v[12]), "+v"(v[13]), "+v"(v[14]), "+v"(v[15])       \
-      : "v"(pair))
-  if constexpr (CTRL == kDppXor1) TQ_PAIRS("quad_perm:[1,0,3,2]");
-  if constexpr (CTRL == kDppXor2) TQ_PAIRS("quad_perm:[2,3,0,1]");
-  if constexpr (CTRL == kDppHalfMirror) TQ_PAIRS("row_half_mirror");
-  if constexpr (CTRL == kDppRor8) TQ_PAIRS("row_ror:8");
-#undef TQ_PAIRS
-#undef TQ_PAIR
-}
-
 constexpr int kAppendBuckets = 64;
 // Rows (of all streams) up to which append_few_kernel runs: append_kernel's
 // tables cost 1.5 to 3 us, its rows less than half.  The lines lie where the
