@@ -19,12 +19,6 @@ using namespace tq;
 
 namespace {
 
-// Whether rows of 8 elements from `p`, strides apart, are 16-byte aligned.
-bool vectors(const void* p, int type, int64_t s0, int64_t s1) {
-  const int64_t size = type == TQ_F32 ? 4 : 2;
-  return aligned16(p) && s0 * size % 16 == 0 && s1 * size % 16 == 0;
-}
-
 // Heads to a workgroup of an append, which share their tokens' table entries: as
 // many (8 at most) as leave this many workgroups.
 constexpr int64_t kAppendBlocks = 1024;

@@ -3,6 +3,7 @@
 //
 // Kernels
 //   paged_split_kernel   attention of few rows over long contexts
+//   paged_chunk_kernel   attention of many rows
 //   paged_merge_kernel   the parts of rows whose keys were cut, as one
 
 #include <hip/hip_runtime.h>
@@ -10,7 +11,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "paged_attention.hpp"
+#include "paged_chunk.hpp"
 #include "paged_host.hpp"
 
 using namespace tq;
@@ -20,6 +21,8 @@ namespace {
 // How a call's attention is cut: `items` units of R rows, `workgroups` to a KV
 // head (0: a workgroup to an item and no merge).
 struct PagedPlan {
+  bool chunk;  // paged_chunk_kernel
+  int rows;    // R
   int64_t items;
   int workgroups;
   size_t acc_bytes, ml_bytes, cut_bytes;
@@ -30,42 +33,62 @@ constexpr int kLeastTiles = 8;  // tiles of 64 keys that a workgroup takes at le
 
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
+// Rows (tokens x group) of a sequence from which the chunk kernel runs.
+constexpr int64_t kChunkFrom = 48;
+
 PagedPlan plan_attention(int64_t tokens, int batch, bool ragged, int group, int kv_heads, int head_dim, int max_pages,
-                         int page_size, int num_cus) {
+                         int page_size, int64_t max_tokens, int num_cus) {
   PagedPlan p{};
-  p.items = ragged ? tokens * group / kSplitRows + batch : static_cast<int64_t>(batch) * ((group + kSplitRows - 1) / kSplitRows);
+  if (!ragged) max_tokens = 1;
+  if (max_tokens <= 0) max_tokens = (tokens + batch - 1) / batch;  // unknown: as if all had as many
+  p.chunk = std::min(max_tokens, tokens) * group >= kChunkFrom;
+  p.rows = p.chunk ? kChunkRows : kSplitRows;
+  p.items = ragged ? tokens * group / p.rows + batch : static_cast<int64_t>(batch) * ((group + p.rows - 1) / p.rows);
   const int64_t tiles = (static_cast<int64_t>(max_pages) * page_size + kTile - 1) / kTile;  // of one sequence, at most
   const int64_t units = p.items * kv_heads;
-  if (tiles <= kLeastTiles || units >= 16 * static_cast<int64_t>(num_cus)) return p;
-  const int64_t fill = std::max<int64_t>(1, 2 * static_cast<int64_t>(num_cus) / kv_heads);
-  const int64_t most = std::max<int64_t>(1, (p.items * std::max<int64_t>(tiles, 1) + kLeastTiles - 1) / kLeastTiles);
+  if (tiles <= kLeastTiles || units >= (p.chunk ? 1 : 16) * static_cast<int64_t>(num_cus)) return p;
+  const int64_t fill = std::max<int64_t>(1, (p.chunk && head_dim == 256 ? 1 : 2) * static_cast<int64_t>(num_cus) / kv_heads);
+  const int64_t most = std::max<int64_t>(1, (p.items * tiles + kLeastTiles - 1) / kLeastTiles);
   p.workgroups = static_cast<int>(std::min(fill, most));
-  const size_t slots = static_cast<size_t>(p.workgroups) * kv_heads * 2 * kSplitRows;
+  const size_t slots = static_cast<size_t>(p.workgroups) * kv_heads * 2 * p.rows;
   p.acc_bytes = align256(slots * head_dim * sizeof(float));
   p.ml_bytes = align256(slots * 2 * sizeof(float));
   p.cut_bytes = align256(static_cast<size_t>(p.items) * kv_heads * sizeof(int2));
   return p;
 }
 
+// The attention kernel over the plan's workgroups, and the merge where keys are cut.
 template <int D, int PLANES>
-int launch_split(const PagedAttentionArgs& a, const PagedPlan& plan, hipStream_t stream) {
+int launch_planned(const PagedAttentionArgs& a, const PagedPlan& plan, hipStream_t stream) {
   const unsigned heads = static_cast<unsigned>(a.batch.kv_heads);
+  const char* name = plan.chunk ? "paged_chunk_kernel" : "paged_split_kernel";
+  const dim3 grid(static_cast<unsigned>(plan.workgroups == 0 ? plan.items : plan.workgroups), heads);
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(plan.chunk ? chunk_threads(D) : kBlock), 0, stream, a); };
   if (plan.workgroups == 0) {
-    hipLaunchKernelGGL((paged_split_kernel<D, PLANES, false>), dim3(static_cast<unsigned>(plan.items), heads), dim3(kBlock), 0, stream, a);
-    return launch_status("paged_split_kernel");
+    if (plan.chunk)
+      launch(paged_chunk_kernel<D, PLANES - 1, false>);
+    else
+      launch(paged_split_kernel<D, PLANES, false>);
+    return launch_status(name);
   }
-  hipLaunchKernelGGL((paged_split_kernel<D, PLANES, true>), dim3(static_cast<unsigned>(plan.workgroups), heads), dim3(kBlock), 0, stream, a);
-  const int rc = launch_status("paged_split_kernel");
+  if (plan.chunk)
+    launch(paged_chunk_kernel<D, PLANES - 1, true>);
+  else
+    launch(paged_split_kernel<D, PLANES, true>);
+  const int rc = launch_status(name);
   if (rc) return rc;
   const int64_t rows = static_cast<int64_t>(a.batch.tokens) * heads * a.group;
-  hipLaunchKernelGGL((paged_merge_kernel<D, kSplitRows>), dim3(static_cast<unsigned>((rows + kWavesPerBlock - 1) / kWavesPerBlock)),
-                     dim3(kBlock), 0, stream, a);
+  const dim3 merge(static_cast<unsigned>((rows + kWavesPerBlock - 1) / kWavesPerBlock));
+  if (plan.chunk)
+    hipLaunchKernelGGL((paged_merge_kernel<D, kChunkRows>), merge, dim3(kBlock), 0, stream, a);
+  else
+    hipLaunchKernelGGL((paged_merge_kernel<D, kSplitRows>), merge, dim3(kBlock), 0, stream, a);
   return launch_status("paged_merge_kernel");
 }
 
 template <int D>
 int launch_attention_d(const PagedAttentionArgs& a, const PagedPlan& plan, hipStream_t stream) {
-  return a.query_type == TQ_F32 ? launch_split<D, 3>(a, plan, stream) : launch_split<D, 2>(a, plan, stream);
+  return a.query_type == TQ_F32 ? launch_planned<D, 3>(a, plan, stream) : launch_planned<D, 2>(a, plan, stream);
 }
 
 }  // namespace
@@ -78,8 +101,7 @@ size_t tq_paged_attention_workspace_bytes(int64_t tokens, int batch, int ragged,
       check_pages(1, page_size, kv_heads, head_dim) != TQ_OK)
     return 0;
   if (num_cus <= 0) num_cus = device_cu_count();
-  (void)max_tokens;
-  const PagedPlan p = plan_attention(tokens, batch, ragged != 0, query_heads / kv_heads, kv_heads, head_dim, max_pages, page_size, num_cus);
+  const PagedPlan p = plan_attention(tokens, batch, ragged != 0, query_heads / kv_heads, kv_heads, head_dim, max_pages, page_size, max_tokens, num_cus);
   return p.acc_bytes + p.ml_bytes + p.cut_bytes;
 }
 
@@ -103,7 +125,7 @@ int tq_paged_attention(const void* query, int64_t query_token_stride, int64_t qu
     return fail(TQ_ERR_BAD_ARG, "null pointer argument");
   if (!aligned16(key_pages) || !aligned16(value_pages)) return fail(TQ_ERR_BAD_ARG, "pages must be 16-byte aligned");
   const int group = query_heads / kv_heads;
-  const PagedPlan plan = plan_attention(tokens, batch, token_starts != nullptr, group, kv_heads, head_dim, max_pages, page_size, device_cu_count());
+  const PagedPlan plan = plan_attention(tokens, batch, token_starts != nullptr, group, kv_heads, head_dim, max_pages, page_size, max_tokens, device_cu_count());
   if (plan.items > INT_MAX) return fail(TQ_ERR_BAD_ARG, "tokens x group exceeds one launch");
   const size_t need = plan.acc_bytes + plan.ml_bytes + plan.cut_bytes;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
@@ -115,6 +137,8 @@ int tq_paged_attention(const void* query, int64_t query_token_stride, int64_t qu
   a.query_type = query_dtype;
   a.q_token_stride = query_token_stride;
   a.q_head_stride = query_head_stride;
+  a.o_vec = vectors(out, query_dtype, out_token_stride, out_head_stride);
+  a.q_vec = vectors(query, query_dtype, query_token_stride, query_head_stride);
   a.out = out;
   a.o_token_stride = out_token_stride;
   a.o_head_stride = out_head_stride;

@@ -22,8 +22,10 @@ struct PagedAttentionArgs {
   const void* query;  // [tokens, query_heads, D], unit stride along D
   int query_type;
   int64_t q_token_stride, q_head_stride;
+  int q_vec;  // eight elements are 16-byte aligned
   void* out;  // the query's type
   int64_t o_token_stride, o_head_stride;
+  int o_vec;
   int group;  // query heads to a KV head
   const int8_t* key_pages;
   const int8_t* value_pages;
@@ -204,6 +206,57 @@ __device__ __forceinline__ uint32_t byte_of_each(uint32_t a, uint32_t b, uint32_
   return __builtin_amdgcn_perm(b, a, pick) | (__builtin_amdgcn_perm(d, c, pick) << 16);
 }
 
+// 16 consecutive elements of a query row (zeros where there is none).
+__device__ __forceinline__ void paged_query16(const PagedAttentionArgs& a, int64_t at, bool live, float (&x)[16]) {
+  if (live) {
+    load8<kAnyRows>(a.query, at, a.query_type, a.q_vec, x);
+    load8<kAnyRows>(a.query, at + 8, a.query_type, a.q_vec, x + 8);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+  }
+}
+// Four consecutive elements of the output, at a multiple of 4 of a row.
+__device__ __forceinline__ void paged_store4(const PagedAttentionArgs& a, int64_t at, const float (&v)[4]) {
+  if (!a.o_vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_as(a.out, at + i, v[i], a.query_type);
+  } else if (a.query_type == kTypeF32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) =
+        make_uint2(two_halves(v[0], v[1], a.query_type), two_halves(v[2], v[3], a.query_type));
+  }
+}
+__device__ __forceinline__ void paged_extent(const float (&x)[16], float* top, bool* fine) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    *top = fmaxf(*top, fabsf(x[i]));
+    *fine = *fine && fabsf(x[i]) < INFINITY;
+  }
+}
+// Their products with f, rounded, in PLANES balanced base-256 digits, the highest first.
+template <int PLANES>
+__device__ __forceinline__ void paged_digits(const float (&x)[16], float f, bool bad, PagedI4 (&q)[PLANES]) {
+  constexpr float kUnit = PLANES == 3 ? 8323072.f : 32512.f;  // 127 x 256^(PLANES-1)
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t digit[PLANES] = {};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      int n = bad ? 0 : static_cast<int>(fminf(fmaxf(rintf(x[4 * w + e] * f), -kUnit), kUnit));
+#pragma unroll
+      for (int k = PLANES - 1; k >= 0; --k) {
+        const int d = k == 0 ? n : static_cast<int8_t>(n);
+        digit[k] |= static_cast<uint32_t>(d & 0xff) << (8 * e);
+        n = (n - d) >> 8;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < PLANES; ++k) q[k][w] = static_cast<int>(digit[k]);
+  }
+}
+
 // paged_split_kernel<D, PLANES>: few rows (single tokens, drafts) over long
 // contexts; one wavefront takes every fourth tile of 64 keys by itself, straight
 // from memory to the matrix instructions' operands.
@@ -248,36 +301,21 @@ __global__ __launch_bounds__(kBlock, 2) void paged_split_kernel(const PagedAtten
       float top = 0.f;
       bool fine = true;
 #pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          x[c][e] = live ? load_as_f32(a.query, base + 64 * c + 16 * g + e, a.query_type) : 0.f;
-          top = fmaxf(top, fabsf(x[c][e]));
-          fine = fine && fabsf(x[c][e]) < INFINITY;
-        }
+      for (int c = 0; c < C; ++c) {
+        paged_query16(a, base + 64 * c + 16 * g, live, x[c]);
+        paged_extent(x[c], &top, &fine);
+      }
       top = xor_reduce<32, OpMax>(xor_reduce<16, OpMax>(top));
-      const float bad = xor_reduce<32, OpMax>(xor_reduce<16, OpMax>(fine ? 0.f : 1.f));
+      const bool bad = xor_reduce<32, OpMax>(xor_reduce<16, OpMax>(fine ? 0.f : 1.f)) > 0.f;
       const float f = top > 1e-30f ? kUnit / top : 0.f;
-      unit = bad > 0.f ? NAN : (top > 1e-30f ? top / kUnit : 0.f) * a.score_scale;
+      unit = bad ? NAN : (top > 1e-30f ? top / kUnit : 0.f) * a.score_scale;
 #pragma unroll
-      for (int c = 0; c < C; ++c)
+      for (int c = 0; c < C; ++c) {
+        PagedI4 d[PLANES];
+        paged_digits<PLANES>(x[c], f, bad, d);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t digit[PLANES] = {};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y = fminf(fmaxf(rintf(x[c][4 * w + e] * f), -kUnit), kUnit);
-            int n = bad > 0.f ? 0 : static_cast<int>(y);
-#pragma unroll
-            for (int k = PLANES - 1; k >= 0; --k) {
-              const int d = k == 0 ? n : static_cast<int8_t>(n);
-              digit[k] |= static_cast<uint32_t>(d & 0xff) << (8 * e);
-              n = (n - d) >> 8;
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < PLANES; ++k) q[k][c][w] = static_cast<int>(digit[k]);
-        }
+        for (int k = 0; k < PLANES; ++k) q[k][c] = d[k];
+      }
     }
     const int64_t keys = live ? at.keys : 0;
 

@@ -98,4 +98,65 @@ __device__ __forceinline__ float paged_scale(float largest) {
   return fmaxf(ldexpf(1.f, e - 7 + (m > 127.f / 128.f ? 1 : 0)), 0x1p-40f);
 }
 
+// ---- rows of a model's tensors
+
+// What a kernel knows of its rows when it is compiled: their type (16-byte
+// aligned, float32 tables, eight elements' partners side by side), or nothing.
+constexpr int kAnyRows = 3;
+
+__device__ __forceinline__ void two_floats(uint32_t w, int type, float* v) {
+  if (type == kTypeF16) {
+    v[0] = __half2float(__ushort_as_half(static_cast<uint16_t>(w)));
+    v[1] = __half2float(__ushort_as_half(static_cast<uint16_t>(w >> 16)));
+  } else {
+    v[0] = __uint_as_float(w << 16);
+    v[1] = __uint_as_float(w & 0xffff0000u);
+  }
+}
+
+// Eight consecutive elements; `vec`: they are 16-byte aligned.
+template <int KIND>
+__device__ __forceinline__ void load8(const void* p, int64_t at, int type, bool vec, float* v) {
+  if constexpr (KIND != kAnyRows) type = KIND, vec = true;
+  if (vec && type == kTypeF32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    const float4 a = q[0], b = q[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else if (vec) {
+    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) two_floats(w[i], type, v + 2 * i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = load_as_f32(p, at + i, type);
+  }
+}
+
+typedef float PagedF2 __attribute__((ext_vector_type(2)));
+typedef _Float16 PagedH2 __attribute__((ext_vector_type(2)));
+typedef __bf16 PagedB2 __attribute__((ext_vector_type(2)));
+
+// Two values in 16 bits each, rounded to nearest even (one instruction either way).
+__device__ __forceinline__ uint32_t two_halves(float lo, float hi, int type) {
+  const PagedF2 v = {lo, hi};
+  return type == kTypeF16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(v, PagedH2))
+                          : __builtin_bit_cast(uint32_t, __builtin_convertvector(v, PagedB2));
+}
+
+template <int KIND>
+__device__ __forceinline__ void store8(void* p, int64_t at, int type, const float* v) {  // 16-byte aligned
+  if constexpr (KIND != kAnyRows) type = KIND;
+  if (type == kTypeF32) {
+    float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+    q[0] = make_float4(v[0], v[1], v[2], v[3]);
+    q[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = two_halves(v[2 * i], v[2 * i + 1], type);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 }  // namespace tq

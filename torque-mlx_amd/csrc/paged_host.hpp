@@ -57,4 +57,11 @@ inline int check_heads(int64_t tokens, int query_heads, int kv_heads) {
   return TQ_OK;
 }
 
+
+// Whether rows of 8 elements from `p`, strides apart, are 16-byte aligned.
+inline bool vectors(const void* p, int type, int64_t s0, int64_t s1) {
+  const int64_t size = type == TQ_F32 ? 4 : 2;
+  return aligned16(p) && s0 * size % 16 == 0 && s1 * size % 16 == 0;
+}
+
 }  // namespace tq
