@@ -47,7 +47,7 @@ PagedPlan plan_attention(int64_t tokens, int batch, bool ragged, int group, int 
   const int64_t tiles = (static_cast<int64_t>(max_pages) * page_size + kTile - 1) / kTile;  // of one sequence, at most
   const int64_t units = p.items * kv_heads;
   if (tiles <= kLeastTiles || units >= (p.chunk ? 1 : 16) * static_cast<int64_t>(num_cus)) return p;
-  const int64_t fill = std::max<int64_t>(1, (p.chunk && head_dim == 256 ? 1 : 2) * static_cast<int64_t>(num_cus) / kv_heads);
+  const int64_t fill = std::max<int64_t>(1, (p.chunk ? (head_dim == 256 ? 1 : 2) : 1) * static_cast<int64_t>(num_cus) / kv_heads);
   const int64_t most = std::max<int64_t>(1, (p.items * tiles + kLeastTiles - 1) / kLeastTiles);
   p.workgroups = static_cast<int>(std::min(fill, most));
   const size_t slots = static_cast<size_t>(p.workgroups) * kv_heads * 2 * p.rows;
@@ -63,7 +63,7 @@ int launch_planned(const PagedAttentionArgs& a, const PagedPlan& plan, hipStream
   const unsigned heads = static_cast<unsigned>(a.batch.kv_heads);
   const char* name = plan.chunk ? "paged_chunk_kernel" : "paged_split_kernel";
   const dim3 grid(static_cast<unsigned>(plan.workgroups == 0 ? plan.items : plan.workgroups), heads);
-  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(plan.chunk ? chunk_threads(D) : kBlock), 0, stream, a); };
+  const auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(plan.chunk ? chunk_threads(D) : split_waves(D) * kWave), 0, stream, a); };
   if (plan.workgroups == 0) {
     if (plan.chunk)
       launch(paged_chunk_kernel<D, PLANES - 1, false>);
@@ -80,9 +80,11 @@ int launch_planned(const PagedAttentionArgs& a, const PagedPlan& plan, hipStream
   const int64_t rows = static_cast<int64_t>(a.batch.tokens) * heads * a.group;
   const dim3 merge(static_cast<unsigned>((rows + kWavesPerBlock - 1) / kWavesPerBlock));
   if (plan.chunk)
-    hipLaunchKernelGGL((paged_merge_kernel<D, kChunkRows>), merge, dim3(kBlock), 0, stream, a);
+    hipLaunchKernelGGL((paged_merge_kernel<D, kChunkRows, 1>), merge, dim3(kBlock), 0, stream, a);
+  else if (plan.workgroups < 8 * plan.items)  // fewer than 8 parts to a row, by and large
+    hipLaunchKernelGGL((paged_merge_kernel<D, kSplitRows, 1>), merge, dim3(kBlock), 0, stream, a);
   else
-    hipLaunchKernelGGL((paged_merge_kernel<D, kSplitRows>), merge, dim3(kBlock), 0, stream, a);
+    hipLaunchKernelGGL((paged_merge_kernel<D, kSplitRows, kWavesPerBlock>), dim3(static_cast<unsigned>(rows)), dim3(kBlock), 0, stream, a);
   return launch_status("paged_merge_kernel");
 }
 

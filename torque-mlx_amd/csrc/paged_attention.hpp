@@ -92,28 +92,14 @@ __device__ __forceinline__ PagedItem paged_item(const PagedAttentionArgs& a, int
 // sees nothing, so that somebody writes its zeros.
 __device__ __forceinline__ int paged_cost(const PagedItem& it) { return it.rows == 0 ? 0 : max(it.tiles, 1); }
 
-// Sum over the workgroup, the same in every thread; `before` is the sum of the
-// threads before this one.
-template <int WAVES>
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* before, int64_t* s_wave) {
-  int64_t sum = v;
+// Sum of the lanes up to and with this one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
-    const int64_t other = __shfl_up(sum, d);
-    if (lane_id() >= d) sum += other;
+    const uint32_t other = static_cast<uint32_t>(__shfl_up(static_cast<int>(v), d));
+    if (lane_id() >= d) v += other;
   }
-  const int wave = threadIdx.x >> 6;
-  __syncthreads();
-  if (lane_id() == kWave - 1) s_wave[wave] = sum;
-  __syncthreads();
-  int64_t base = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    if (w < wave) base += s_wave[w];
-    total += s_wave[w];
-  }
-  *before = base + sum - v;
-  return total;
+  return v;
 }
 
 // Runs work(item, index, from, to, whole, slot) for each part of an item that
@@ -126,50 +112,48 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* before, int64_
 // item leaves its sums in the workgroup's slot 0 (an item begun before) or 1 (an
 // item that it begins), for the merge.
 // Otherwise workgroup x has item x.
-template <int R, bool CUT, int WAVES, class Work>
+//
+// Every wavefront finds its workgroup's run by itself, 64 items at a time, without
+// a barrier: the lengths are the first load of the call, and all else waits for them.
+template <int R, bool CUT, class Work>
 __device__ __forceinline__ void paged_schedule(const PagedAttentionArgs& a, int h, Work work) {
   if constexpr (!CUT) {
     const int index = a.items - 1 - static_cast<int>(blockIdx.x);  // a sequence's last rows see the most keys
     const PagedItem it = paged_item<R>(a, index);
     if (it.rows > 0) work(it, 0, it.tiles, true, 0);
   } else {
-    __shared__ int64_t s_wave[WAVES];
-    __shared__ int s_index;
-    __shared__ int64_t s_offset;
-    constexpr int N = WAVES * kWave;
-    const int workgroups = gridDim.x, tid = threadIdx.x;
-    int64_t total = 0, before = 0;
-    int64_t mine = 0;
-    for (int i0 = 0; i0 < a.items; i0 += N)
-      if (i0 + tid < a.items) mine += paged_cost(paged_item<R>(a, i0 + tid));
-    total = block_scan<WAVES>(mine, &before, s_wave);
+    const int workgroups = gridDim.x, lane = lane_id();
+    auto cost_of = [&](int index) { return index < a.items ? static_cast<uint32_t>(paged_cost(paged_item<R>(a, index))) : 0u; };
+    uint32_t mine = cost_of(lane), sum = wave_scan(mine);
+    int64_t total = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum), 63));
+    for (int i0 = kWave; i0 < a.items; i0 += kWave)
+      total += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan(cost_of(i0 + lane))), 63));
     const int64_t run = max((total + workgroups - 1) / workgroups, static_cast<int64_t>(a.least_tiles));
     int64_t at = run * blockIdx.x;
     const int64_t end = min(at + run, total);
     if (at >= end) return;
-    if (tid == 0) s_index = a.items;  // nothing to do, were no item found
-    int64_t base = 0;
-    for (int i0 = 0; i0 < a.items; i0 += N) {
-      const int64_t cost = i0 + tid < a.items ? paged_cost(paged_item<R>(a, i0 + tid)) : 0;
-      const int64_t all = block_scan<WAVES>(cost, &before, s_wave);
-      if (at < base + all) {  // the same in every thread
-        if (at >= base + before && at < base + before + cost) {
-          s_index = i0 + tid;
-          s_offset = at - base - before;
-        }
+    int index = a.items;  // nothing to do, were no item found
+    int64_t offset = 0, base = 0;
+    for (int i0 = 0; i0 < a.items; i0 += kWave) {
+      if (i0 > 0) {
+        mine = cost_of(i0 + lane);
+        sum = wave_scan(mine);
+      }
+      const uint32_t all = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum), 63));
+      if (at < base + all) {  // the item that holds tile `at`: the first whose sum passes it
+        const int k = __ffsll(__ballot(base + sum > at)) - 1;
+        index = i0 + k;
+        offset = at - base - static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum - mine), k));
         break;
       }
       base += all;
     }
-    __syncthreads();
-    int index = s_index;
-    int64_t offset = s_offset;
     while (at < end && index < a.items) {
       const PagedItem it = paged_item<R>(a, index);
       const int cost = paged_cost(it);
       if (cost > 0) {
         const int64_t take = min(cost - offset, end - at);
-        if (offset == 0 && tid == 0) {
+        if (offset == 0 && threadIdx.x == 0) {
           const int64_t first = at / run, last = (at + cost - 1) / run;
           a.cut[static_cast<int64_t>(index) * a.batch.kv_heads + h] =
               make_int2(static_cast<int>(first), last > first ? static_cast<int>(last - first + 1) : 0);
@@ -200,12 +184,6 @@ __device__ __forceinline__ PagedRowAt paged_row(const PagedAttentionArgs& a, con
   return at;
 }
 
-// The bytes k of four words as one word.
-__device__ __forceinline__ uint32_t byte_of_each(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int k) {
-  const uint32_t pick = 0x0C0C0400u + 0x00000101u * k;  // (second operand's byte k, first operand's byte k)
-  return __builtin_amdgcn_perm(b, a, pick) | (__builtin_amdgcn_perm(d, c, pick) << 16);
-}
-
 // 16 consecutive elements of a query row (zeros where there is none).
 __device__ __forceinline__ void paged_query16(const PagedAttentionArgs& a, int64_t at, bool live, float (&x)[16]) {
   if (live) {
@@ -228,37 +206,54 @@ __device__ __forceinline__ void paged_store4(const PagedAttentionArgs& a, int64_
         make_uint2(two_halves(v[0], v[1], a.query_type), two_halves(v[2], v[3], a.query_type));
   }
 }
-__device__ __forceinline__ void paged_extent(const float (&x)[16], float* top, bool* fine) {
+// Bits of the largest of |x| and `top` (an infinity, a NaN above all).
+__device__ __forceinline__ uint32_t paged_extent(const float (&x)[16], uint32_t top) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    *top = fmaxf(*top, fabsf(x[i]));
-    *fine = *fine && fabsf(x[i]) < INFINITY;
-  }
+  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  return top;
 }
-// Their products with f, rounded, in PLANES balanced base-256 digits, the highest first.
+
+// The bytes k of four words as one word.
+__device__ __forceinline__ uint32_t byte_of_each(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int k) {
+  const uint32_t pick = 0x0C0C0400u + 0x00000101u * k;  // (second operand's byte k, first operand's byte k)
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, pick), __builtin_amdgcn_perm(b, a, pick), 0x05040100u);
+}
+
+// Integers n = x f, rounded, |n| <= kQueryUnit, in PLANES balanced base-256 digits,
+// the highest first.  The sum with 2^23 and an offset rounds them and leaves
+// n + offset in the mantissa's low bits, whose bytes are the digits, each off by
+// what the offset has there: 128, and 64 at the top of three (2^22 + 32896 in all).
 template <int PLANES>
-__device__ __forceinline__ void paged_digits(const float (&x)[16], float f, bool bad, PagedI4 (&q)[PLANES]) {
-  constexpr float kUnit = PLANES == 3 ? 8323072.f : 32512.f;  // 127 x 256^(PLANES-1)
+constexpr float kQueryUnit = PLANES == 3 ? 4161280.f : 32512.f;  // with the offset below 2^23, and below 2^16
+template <int PLANES>
+__device__ __forceinline__ void paged_digits(const float (&x)[16], float f, PagedI4 (&q)[PLANES]) {
+  constexpr float kMagic = 8388608.f + (PLANES == 3 ? 4194304.f + 32896.f : 32768.f + 128.f);
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    uint32_t digit[PLANES] = {};
+    uint32_t n[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      int n = bad ? 0 : static_cast<int>(fminf(fmaxf(rintf(x[4 * w + e] * f), -kUnit), kUnit));
+    for (int e = 0; e < 4; ++e) n[e] = __float_as_uint(fmaf(x[4 * w + e], f, kMagic));
 #pragma unroll
-      for (int k = PLANES - 1; k >= 0; --k) {
-        const int d = k == 0 ? n : static_cast<int8_t>(n);
-        digit[k] |= static_cast<uint32_t>(d & 0xff) << (8 * e);
-        n = (n - d) >> 8;
-      }
+    for (int k = 0; k < PLANES; ++k) {
+      const uint32_t bytes = byte_of_each(n[0], n[1], n[2], n[3], PLANES - 1 - k);
+      if (PLANES == 3 && k == 0)  // less 64: bytes below 128 with the sign bit set leave no borrow
+        q[k][w] = static_cast<int>(((bytes | 0x80808080u) - 0x40404040u) ^ 0x80808080u);
+      else
+        q[k][w] = static_cast<int>(bytes ^ 0x80808080u);
     }
-#pragma unroll
-    for (int k = 0; k < PLANES; ++k) q[k][w] = static_cast<int>(digit[k]);
   }
+}
+// What digits are multiplied back by, and what elements are multiplied with: NaN
+// for a row with an element that is not finite, 0 for one (of almost) nothing.
+template <int PLANES>
+__device__ __forceinline__ float paged_unit(uint32_t top, float* f) {
+  const float t = __uint_as_float(top);
+  *f = t > 1e-30f && t < INFINITY ? kQueryUnit<PLANES> / t : 0.f;
+  return !(t < INFINITY) ? NAN : t > 1e-30f ? t / kQueryUnit<PLANES> : 0.f;
 }
 
 // paged_split_kernel<D, PLANES>: few rows (single tokens, drafts) over long
-// contexts; one wavefront takes every fourth tile of 64 keys by itself, straight
+// contexts; one wavefront takes every eighth tile of 64 keys by itself, straight
 // from memory to the matrix instructions' operands.
 //
 // The codes are multiplied as they are, in v_mfma_i32_16x16x64_i8.  A query row
@@ -276,43 +271,83 @@ __device__ __forceinline__ void paged_digits(const float (&x)[16], float f, bool
 // (column j, g = lane / 16) then holds the scores of tokens 16 g .. 16 g + 15,
 // which is what it needs as the second product's right operand: 16 bytes of
 // weights for 16 bytes of values that lie side by side in the transposed page.
+//
+// A wavefront's next keys are on their way from the moment the current ones are
+// multiplied, its next values likewise, and page numbers a tile before that.
+constexpr int split_waves(int d) { return d == 256 ? 4 : 8; }
+
 template <int D, int PLANES, bool CUT>
-__global__ __launch_bounds__(kBlock, 2) void paged_split_kernel(const PagedAttentionArgs a) {
-  constexpr int R = 16, C = D / 64, DT = D / 16;
+__global__ __launch_bounds__(split_waves(D) * kWave, (D == 256 ? 1 : 2)) void paged_split_kernel(const PagedAttentionArgs a) {
+  constexpr int R = 16, C = D / 64, DT = D / 16, kSplitWaves = split_waves(D);
   constexpr int P = D + 4;  // LDS pitch of a row of sums
   constexpr float kUnit = PLANES == 3 ? 8323072.f : 32512.f;  // 127 x 256^(PLANES-1)
-  __shared__ float s_acc[kWavesPerBlock][R][P];
-  __shared__ float s_ml[kWavesPerBlock][R][2];
+  __shared__ __align__(16) float s_acc[kSplitWaves][R][P];
+  __shared__ float s_ml[kSplitWaves][R][2];
   const PagedBatch& p = a.batch;
   const int lane = lane_id(), wave = threadIdx.x >> 6;
   const int j = lane & 15, g = lane >> 4;
   const int h = blockIdx.y;
   const int T = 1 << p.log_page;
 
-  paged_schedule<R, CUT, kWavesPerBlock>(a, h, [&](const PagedItem& it, int from, int to, bool whole, int slot) {
-    // ---- this lane's query row, 16 dimensions of each chunk of 64
+  paged_schedule<R, CUT>(a, h, [&](const PagedItem& it, int from, int to, bool whole, int slot) {
+    // ---- page numbers: this lane's key rows are in group j / 4 of a tile's 16 tokens, its values and scores in group g
+    auto page_of = [&](int tile, int group) {
+      const int64_t t = static_cast<int64_t>(tile) * kTile + 16 * group;
+      return tile < to && t < it.s.len ? paged_page(p, it.b, t >> p.log_page) : -1;
+    };
+    PagedI4 kv[4][C], vv[DT];
+    float ks, vs;
+    auto load_keys = [&](int tile, int id) {
+      const int64_t page = static_cast<int64_t>(max(id, 0)) * p.kv_heads + h;
+      const int first = (tile * kTile + 16 * (j >> 2)) & (T - 1);
+      const int8_t* kp = a.key_pages + page * (D << p.log_page) + (first + (j & 3)) * D + 16 * g;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int c = 0; c < C; ++c) kv[s][c] = *reinterpret_cast<const PagedI4*>(kp + 4 * s * D + 64 * c);
+    };
+    auto load_values = [&](int tile, int id) {
+      const int64_t page = static_cast<int64_t>(max(id, 0)) * p.kv_heads + h;
+      const int8_t* vp = a.value_pages + page * (D << p.log_page) + ((tile * kTile + 16 * g) & (T - 1)) + j * T;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) vv[t] = *reinterpret_cast<const PagedI4*>(vp + 16 * t * T);
+    };
+    auto load_scales = [&](int id) {
+      const int64_t page = static_cast<int64_t>(max(id, 0)) * p.kv_heads + h;
+      ks = a.key_scales[page];
+      vs = a.value_scales[page];
+    };
+    // The query row's load goes first: loads return in order, and its digits are made while keys are on their way.
     const bool live = j < it.rows;
     const PagedRowAt at = paged_row(a, it, h, live ? j : 0);
+    float x[C][16];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      paged_query16(a, at.token * a.q_token_stride + at.head * a.q_head_stride + 64 * c + 16 * g, live, x[c]);
+    int tile = from + wave;
+    int vid = page_of(tile, g), knext = -1, vnext = -1;
+    if (tile < to) {
+      const int kid = page_of(tile, j >> 2);
+      knext = page_of(tile + kSplitWaves, j >> 2);
+      vnext = page_of(tile + kSplitWaves, g);
+      load_keys(tile, kid);
+      load_scales(vid);
+      load_values(tile, vid);
+    }
+    // ---- this lane's query row, 16 dimensions of each chunk of 64
     PagedI4 q[PLANES][C];
     float unit;  // a score is the digits' product times this and the key page's scale
     {
-      const int64_t base = at.token * a.q_token_stride + at.head * a.q_head_stride;
-      float x[C][16];
-      float top = 0.f;
-      bool fine = true;
+      uint32_t top = 0;
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        paged_query16(a, base + 64 * c + 16 * g, live, x[c]);
-        paged_extent(x[c], &top, &fine);
-      }
-      top = xor_reduce<32, OpMax>(xor_reduce<16, OpMax>(top));
-      const bool bad = xor_reduce<32, OpMax>(xor_reduce<16, OpMax>(fine ? 0.f : 1.f)) > 0.f;
-      const float f = top > 1e-30f ? kUnit / top : 0.f;
-      unit = bad ? NAN : (top > 1e-30f ? top / kUnit : 0.f) * a.score_scale;
+      for (int c = 0; c < C; ++c) top = paged_extent(x[c], top);
+      top = __float_as_uint(xor_reduce<32, OpBits>(xor_reduce<16, OpBits>(__uint_as_float(top))));
+      float f;
+      unit = paged_unit<PLANES>(top, &f) * a.score_scale;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         PagedI4 d[PLANES];
-        paged_digits<PLANES>(x[c], f, bad, d);
+        paged_digits<PLANES>(x[c], f, d);
 #pragma unroll
         for (int k = 0; k < PLANES; ++k) q[k][c] = d[k];
       }
@@ -326,26 +361,11 @@ __global__ __launch_bounds__(kBlock, 2) void paged_split_kernel(const PagedAtten
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[t][r] = 0.f;
 
-    for (int tile = from + wave; tile < to; tile += kWavesPerBlock) {
-      const int64_t tok0 = static_cast<int64_t>(tile) * kTile;
-      // key rows of this lane: group i / 4 of 16 tokens; values and scores: group g
-      const int64_t kt = tok0 + 16 * (j >> 2), vt = tok0 + 16 * g;
-      const int kid = kt < it.s.len ? paged_page(p, it.b, kt >> p.log_page) : -1;
-      const int vid = vt < it.s.len ? paged_page(p, it.b, vt >> p.log_page) : -1;
-      const int64_t kpage = static_cast<int64_t>(max(kid, 0)) * p.kv_heads + h;
-      const int64_t vpage = static_cast<int64_t>(max(vid, 0)) * p.kv_heads + h;
-      const int8_t* kp = a.key_pages + kpage * (D << p.log_page) + ((kt & (T - 1)) + (j & 3)) * D + 16 * g;
-      const int8_t* vp = a.value_pages + vpage * (D << p.log_page) + (vt & (T - 1)) + static_cast<int64_t>(j) * T;
-      PagedI4 kv[4][C], vv[DT];
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int c = 0; c < C; ++c) kv[s][c] = *reinterpret_cast<const PagedI4*>(kp + 4 * s * D + 64 * c);
-#pragma unroll
-      for (int t = 0; t < DT; ++t) vv[t] = *reinterpret_cast<const PagedI4*>(vp + 16 * t * T);
-      const float ks = a.key_scales[vpage] * unit;
-      const float vs = a.value_scales[vpage];
-      const float shift = __log2f(vs);
+    for (; tile < to; tile += kSplitWaves) {
+      const int64_t vt = static_cast<int64_t>(tile) * kTile + 16 * g;
+      const int kafter = page_of(tile + 2 * kSplitWaves, j >> 2), vafter = page_of(tile + 2 * kSplitWaves, g);
+      const float by = ks * unit, shift = __log2f(vs), back = 1.f / vs;
+      const int seen = vid >= 0 ? static_cast<int>(min(max(keys - vt, int64_t(0)), int64_t(16))) : 0;  // of its 16 tokens
 
       float w[16];
       float top = -INFINITY;
@@ -366,10 +386,13 @@ __global__ __launch_bounds__(kBlock, 2) void paged_split_kernel(const PagedAtten
         for (int r = 0; r < 4; ++r) {
           float f = static_cast<float>(hi[r]);
           if constexpr (PLANES == 3) f = fmaf(f, 256.f, static_cast<float>(lo[r]));
-          const bool seen = vid >= 0 && vt + 4 * s + r < keys;
-          w[4 * s + r] = seen ? fmaf(f, ks, shift) : -INFINITY;
+          w[4 * s + r] = 4 * s + r < seen ? fmaf(f, by, shift) : -INFINITY;
           top = fmaxf(top, w[4 * s + r]);
         }
+      }
+      if (tile + kSplitWaves < to) {
+        load_keys(tile + kSplitWaves, knext);
+        load_scales(vnext);
       }
       top = xor_reduce<32, OpMax>(xor_reduce<16, OpMax>(top));
       const float base = top == -INFINITY ? 0.f : top;
@@ -384,7 +407,7 @@ __global__ __launch_bounds__(kBlock, 2) void paged_split_kernel(const PagedAtten
       }
       const float next = fmaxf(m, top);
       const float keep = m == next ? 1.f : fast_exp2(m - next), part = top == -INFINITY ? 0.f : fast_exp2(top - next);
-      l = l * keep + (vid >= 0 ? sum * part / vs : 0.f);
+      l = l * keep + (vid >= 0 ? sum * part * back : 0.f);
       m = next;
 
       PagedI4 wq[PLANES];
@@ -410,43 +433,51 @@ __global__ __launch_bounds__(kBlock, 2) void paged_split_kernel(const PagedAtten
           acc[t][r] = fmaf(f, part, acc[t][r] * keep);
         }
       }
+      if (tile + kSplitWaves < to) load_values(tile + kSplitWaves, vnext);
+      vid = vnext;
+      knext = kafter;
+      vnext = vafter;
     }
 
-    // ---- the four wavefronts' sums as one
+    // ---- the wavefronts' sums as one
     l = xor_reduce<32, OpSum>(xor_reduce<16, OpSum>(l));
     __syncthreads();  // the item before is written out
-    if (g == 0) {
-      s_ml[wave][j][0] = m;
-      s_ml[wave][j][1] = l;
+    if (live) {
+      if (g == 0) {
+        s_ml[wave][j][0] = m;
+        s_ml[wave][j][1] = l;
+      }
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+        *reinterpret_cast<float4*>(&s_acc[wave][j][16 * t + 4 * g]) = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
     }
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s_acc[wave][j][16 * t + 4 * g + r] = acc[t][r];
     __syncthreads();
-    for (int i = threadIdx.x; i < R * D; i += kBlock) {
-      const int row = i / D, d = i & (D - 1);
-      if (row >= it.rows) break;
-      float top = -INFINITY, sum = 0.f, weight = 0.f;
+    for (int i = threadIdx.x; i < it.rows * (D / 4); i += kSplitWaves * kWave) {
+      const int row = i / (D / 4), d = 4 * (i & (D / 4 - 1));
+      float top = -INFINITY, weight = 0.f;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int v = 0; v < kWavesPerBlock; ++v) top = fmaxf(top, s_ml[v][row][0]);
+      for (int v = 0; v < kSplitWaves; ++v) top = fmaxf(top, s_ml[v][row][0]);
       const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-      for (int v = 0; v < kWavesPerBlock; ++v) {
+      for (int v = 0; v < kSplitWaves; ++v) {
         const float f = fast_exp2(s_ml[v][row][0] - base);
-        sum = fmaf(s_acc[v][row][d], f, sum);
+        const float4 x = *reinterpret_cast<const float4*>(&s_acc[v][row][d]);
+        sum.x = fmaf(x.x, f, sum.x), sum.y = fmaf(x.y, f, sum.y), sum.z = fmaf(x.z, f, sum.z), sum.w = fmaf(x.w, f, sum.w);
         weight = fmaf(s_ml[v][row][1], f, weight);
       }
-      sum *= 1.f / kUnit;
       if (whole) {
         const PagedRowAt o = paged_row(a, it, h, row);
-        store_as(a.out, o.token * a.o_token_stride + o.head * a.o_head_stride + d, weight == 0.f ? 0.f : sum / weight, a.query_type);
+        const float f = weight == 0.f ? 0.f : 1.f / (weight * kUnit);
+        const float out[4] = {sum.x * f, sum.y * f, sum.z * f, sum.w * f};
+        paged_store4(a, o.token * a.o_token_stride + o.head * a.o_head_stride + d, out);
       } else {
-        const int64_t at_slot = (static_cast<int64_t>(blockIdx.x) * p.kv_heads + h) * 2 + slot;
-        a.acc[(at_slot * R + row) * D + d] = sum;
+        constexpr float f = 1.f / kUnit;
+        const int64_t at_slot = ((static_cast<int64_t>(blockIdx.x) * p.kv_heads + h) * 2 + slot) * R + row;
+        *reinterpret_cast<float4*>(a.acc + at_slot * D + d) = make_float4(sum.x * f, sum.y * f, sum.z * f, sum.w * f);
         if (d == 0) {
-          a.ml[(at_slot * R + row) * 2] = top;
-          a.ml[(at_slot * R + row) * 2 + 1] = weight;
+          a.ml[at_slot * 2] = top;
+          a.ml[at_slot * 2 + 1] = weight;
         }
       }
     }
@@ -454,13 +485,15 @@ __global__ __launch_bounds__(kBlock, 2) void paged_split_kernel(const PagedAtten
 }
 
 // Rows whose keys were cut: the parts' sums, brought to the largest maximum and
-// added in the order of the keys.  One wavefront to a row.
-template <int D, int R>
+// added in a fixed order.  WAVES wavefronts to a row: one, or four that take every
+// fourth part where rows are few and parts many.
+template <int D, int R, int WAVES>
 __global__ __launch_bounds__(kBlock) void paged_merge_kernel(const PagedAttentionArgs a) {
   constexpr int E = D / kWave;
+  __shared__ float s_sum[kWavesPerBlock][D + 2];
   const PagedBatch& p = a.batch;
-  const int heads = p.kv_heads * a.group;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + (threadIdx.x >> 6);
+  const int heads = p.kv_heads * a.group, wave = threadIdx.x >> 6, lane = lane_id();
+  const int64_t row = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave : blockIdx.x;
   if (row >= static_cast<int64_t>(p.tokens) * heads) return;
   const int token = static_cast<int>(row / heads), head = static_cast<int>(row - static_cast<int64_t>(token) * heads);
   const int h = head / a.group;
@@ -473,21 +506,35 @@ __global__ __launch_bounds__(kBlock) void paged_merge_kernel(const PagedAttentio
   const int r = static_cast<int>(local % R);
   const int2 cut = a.cut[item * p.kv_heads + h];
   if (cut.x < 0 || cut.y <= 0 || cut.y > a.workgroups - cut.x) return;  // whole, or (row offsets that decrease) not dealt out
-  const int lane = lane_id();
+  auto slot = [&](int k) { return ((static_cast<int64_t>(cut.x + k) * p.kv_heads + h) * 2 + (k == 0 ? 1 : 0)) * R + r; };
   float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) o[i] = 0.f;
-  auto slot = [&](int k) { return (static_cast<int64_t>(cut.x + k) * p.kv_heads + h) * 2 + (k == 0 ? 1 : 0); };
-  for (int k = lane; k < cut.y; k += kWave) m = fmaxf(m, a.ml[(slot(k) * R + r) * 2]);
+  for (int k = lane; k < cut.y; k += kWave) m = fmaxf(m, a.ml[slot(k) * 2]);
   m = group_reduce<kWave, OpMax>(m);
   if (m == -INFINITY) m = 0.f;
-#pragma unroll 4
-  for (int k = 0; k < cut.y; ++k) {
-    const int64_t at = slot(k) * R + r;
-    const float f = fast_exp2(a.ml[at * 2] - m);
-    l = fmaf(a.ml[at * 2 + 1], f, l);
+#pragma unroll 8
+  for (int k = WAVES == 1 ? 0 : wave; k < cut.y; k += WAVES) {
+    const int64_t at = slot(k);
+    const float2 ml = *reinterpret_cast<const float2*>(a.ml + at * 2);
+    const float f = fast_exp2(ml.x - m);
+    const float* x = a.acc + at * D + lane * E;
+    l = fmaf(ml.y, f, l);
 #pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = fmaf(a.acc[at * D + lane * E + i], f, o[i]);
+    for (int i = 0; i < E; ++i) o[i] = fmaf(x[i], f, o[i]);
+  }
+  if constexpr (WAVES > 1) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) s_sum[wave][lane * E + i] = o[i];
+    if (lane == 0) s_sum[wave][D] = l;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+      l += s_sum[w][D];
+#pragma unroll
+      for (int i = 0; i < E; ++i) o[i] += s_sum[w][lane * E + i];
+    }
   }
 #pragma unroll
   for (int i = 0; i < E; ++i)

@@ -41,16 +41,15 @@ struct HalfScores {
   PagedH8 q[TERMS][D / 16];
 
   __device__ __forceinline__ float set(const PagedAttentionArgs& a, int64_t base, bool live, int g) {
-    float top = 0.f;
-    bool fine = true;
+    uint32_t bits = 0;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       float x[16];
       paged_query16(a, base + 32 * c + 16 * g, live, x);
-      paged_extent(x, &top, &fine);
+      bits = paged_extent(x, bits);
     }
-    top = xor_reduce<32, OpMax>(top);
-    const bool bad = xor_reduce<32, OpMax>(fine ? 0.f : 1.f) > 0.f;
+    const float top = xor_reduce<32, OpBits>(__uint_as_float(bits));
+    const bool bad = !(top < INFINITY);
     int e;
     frexpf(top, &e);
     const float f = top > 1e-30f && !bad ? ldexpf(1.f, 14 - e) : 0.f;
@@ -94,28 +93,26 @@ struct DigitScores {
   PagedI4 q[PLANES][D / 32];
 
   __device__ __forceinline__ float set(const PagedAttentionArgs& a, int64_t base, bool live, int g) {
-    constexpr float kUnit = PLANES == 3 ? 8323072.f : 32512.f;
-    float top = 0.f;
-    bool fine = true;
+    uint32_t top = 0;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       float x[16];
       paged_query16(a, base + 32 * c + 16 * g, live, x);
-      paged_extent(x, &top, &fine);
+      top = paged_extent(x, top);
     }
-    top = xor_reduce<32, OpMax>(top);
-    const bool bad = xor_reduce<32, OpMax>(fine ? 0.f : 1.f) > 0.f;
-    const float f = top > 1e-30f ? kUnit / top : 0.f;
+    top = __float_as_uint(xor_reduce<32, OpBits>(__uint_as_float(top)));
+    float f;
+    const float unit = paged_unit<PLANES>(top, &f) * a.score_scale;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       float x[16];
       paged_query16(a, base + 32 * c + 16 * g, live, x);
       PagedI4 d[PLANES];
-      paged_digits<PLANES>(x, f, bad, d);
+      paged_digits<PLANES>(x, f, d);
 #pragma unroll
       for (int k = 0; k < PLANES; ++k) q[k][c] = d[k];
     }
-    return bad ? NAN : (top > 1e-30f ? top / kUnit : 0.f) * a.score_scale;
+    return unit;
   }
   static __device__ __forceinline__ void put(int8_t* to, int row, int piece, uint4 codes) {
     *reinterpret_cast<uint4*>(to + row * kPitch + 16 * piece) = codes;
@@ -184,7 +181,7 @@ __global__ __launch_bounds__(chunk_threads(D), 2) void paged_chunk_kernel(const 
   const int h = blockIdx.y;
   const int T = 1 << p.log_page;
 
-  paged_schedule<R, CUT, NT / kWave>(a, h, [&](const PagedItem& it, int from, int to, bool whole, int slot) {
+  paged_schedule<R, CUT>(a, h, [&](const PagedItem& it, int from, int to, bool whole, int slot) {
     const int r0 = 32 * (wave & 3), d0 = DH * (wave >> 2);
     const bool live = r0 + j < it.rows;
     const PagedRowAt at = paged_row(a, it, h, live ? r0 + j : 0);
