@@ -20,6 +20,8 @@ from pathlib import Path
 
 import torch
 
+sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "torque-mlx_amd"))
+
 own = False
 
 TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
@@ -300,9 +302,6 @@ def run(s):
 
 
 def _own(s, op):
-    package = str(Path(__file__).resolve().parents[1] / "torque-mlx_amd")
-    if package not in sys.path:
-        sys.path.insert(0, package)
     from torque_hip import ops
 
     pool = {n: s[n] for n in ("key_pages", "value_pages", "key_scales", "value_scales")}
