@@ -4,7 +4,8 @@
     python torque-mlx_amd/build.py --asan OUT.so   # host-only AddressSanitizer build
 
 Compiles the csrc/*.hip sources with hipcc, side by side, and links them into
-torque_hip/libtorque_hip.so, in-tree.  Packed-FP32 VALU ops are disabled for all device code.  The
+torque_hip/libtorque_hip.so, in-tree; csrc/paged_binding.cpp becomes the CPython
+module torque_hip/_paged.so.  Packed-FP32 VALU ops are disabled for all device code.  The
 atomic optimizer is off for device code: it rewrites a single lane's LDS
 atomic (the split kernels' tile counter) into a wave-wide form that waits
 for the result at once, where the kernels want it one iteration later.
@@ -16,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
@@ -24,6 +26,8 @@ ROOT = Path(__file__).resolve().parent
 REPO = ROOT.parent
 SOURCES = tuple(ROOT / "csrc" / name for name in ("torque_hip.hip", "paged_append.hip", "paged_attention.hip"))
 OUTPUT = ROOT / "torque_hip" / "libtorque_hip.so"
+BINDING = ROOT / "csrc" / "paged_binding.cpp"
+BINDING_OUTPUT = ROOT / "torque_hip" / "_paged.so"
 ARCH = os.environ.get("TORQUE_HIP_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
@@ -69,7 +73,7 @@ def _run(cmd: list[str], verbose: bool) -> str:
     noise = "is not a recognized feature for this target"
     stderr = "\n".join(line for line in proc.stderr.splitlines() if noise not in line)
     if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{stderr}")
+        raise RuntimeError(f"{Path(cmd[0]).name} failed ({proc.returncode}):\n{stderr}")
     return stderr
 
 
@@ -93,8 +97,32 @@ def build_library(verbose: bool = False, asan: bool = False, output: Path | None
     return out
 
 
+def build_binding(verbose: bool = False) -> Path:
+    """Compile the paged cache's CPython module (host code over torch's C++ API and the library's C ABI)."""
+    import torch
+
+    base = Path(torch.__path__[0])
+    includes = [base / "include", base / "include/torch/csrc/api/include", "/opt/rocm/include", sysconfig.get_paths()["include"], REPO / "include"]
+    libraries = ["c10", "c10_hip", "torch", "torch_cpu", "torch_hip", "torch_python"]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in includes), str(BINDING), "-o",
+           str(BINDING_OUTPUT) + ".tmp", f"-L{base / 'lib'}", *(f"-l{lib}" for lib in libraries)]
+    _run(cmd, verbose)
+    os.replace(str(BINDING_OUTPUT) + ".tmp", BINDING_OUTPUT)
+    return BINDING_OUTPUT
+
+
+def build_all(verbose: bool = False) -> Path:
+    """The library and the module, side by side."""
+    with ThreadPoolExecutor(1) as pool:
+        binding = pool.submit(build_binding, verbose)
+        library = build_library(verbose)
+        binding.result()
+    return library
+
+
 if __name__ == "__main__":
     if "--asan" in sys.argv:
         print(build_library(verbose=True, asan=True, output=Path(sys.argv[sys.argv.index("--asan") + 1])))
     else:
-        print(build_library(verbose=True))
+        print(build_all(verbose=True))
