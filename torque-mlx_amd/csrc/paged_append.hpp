@@ -130,18 +130,21 @@ __device__ __forceinline__ bool paged_angles(const PagedRotary& r, int l, int64_
 }
 
 // This lane's 16 elements of a row, turned.  Every operation is rounded by itself,
-// as the torch operations of apply_rotary round it in float32.
+// as the torch operations of apply_rotary round it in float32 (one more per
+// element than with a fused multiply-add: keys next to a code's border then have
+// the codes that the composition of torch operations gives them).
 template <int D, int KIND>
 __device__ __forceinline__ void paged_turn(const PagedRotary& r, const PagedRows& x, int64_t base, int l, const float (&c)[16],
                                            const float (&s)[16], float (&v)[16]) {
+#pragma clang fp contract(off)
   constexpr bool PLAIN = KIND != kAnyRows;
   const int half = r.rotary_dim / 2;
   if (r.rotary_dim == D) {  // an element's partner lies in the same lane
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float a = v[i], b = v[8 + i];
-      v[i] = __fadd_rn(__fmul_rn(a, c[i]), __fmul_rn(-b, s[i]));
-      v[8 + i] = __fadd_rn(__fmul_rn(b, c[8 + i]), __fmul_rn(a, s[8 + i]));
+      v[i] = a * c[i] - b * s[i];
+      v[8 + i] = b * c[8 + i] + a * s[8 + i];
     }
     return;
   }
@@ -163,7 +166,7 @@ __device__ __forceinline__ void paged_turn(const PagedRotary& r, const PagedRows
     for (int i = 0; i < 8; ++i) {
       const int d = d0 + (PLAIN ? 0 : i);
       if (!PLAIN && d >= r.rotary_dim) continue;
-      v[8 * h + i] = __fadd_rn(__fmul_rn(v[8 * h + i], c[8 * h + i]), __fmul_rn(d < half ? -w[i] : w[i], s[8 * h + i]));
+      v[8 * h + i] = v[8 * h + i] * c[8 * h + i] + (d < half ? -w[i] : w[i]) * s[8 * h + i];
     }
   }
 }
