@@ -24,6 +24,7 @@ from torque_hip.ops import (
     quantize_and_pack_rows,
     quantize_and_pack_rows_dual,
 )
+from torque_hip.paged_cache import TorquePagedKVCache
 from torque_hip.qwen_benchmark import (
     QwenDecodeBenchmarkProfile,
     QwenDecodeRuntimeBenchmarkResult,
@@ -61,6 +62,7 @@ __all__ = [
     "TorqueKVCache",
     "TorqueKVCacheHIP",
     "TorqueKVCacheMLX",
+    "TorquePagedKVCache",
     "build_gaussian_codebook",
     "build_uniform_codebook",
     "build_variant_id",

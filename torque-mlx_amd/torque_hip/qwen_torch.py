@@ -23,6 +23,12 @@ restores the output projection at run time (qwen_mlx.py:610-618, 773-779);
 starting from a model's own weights, ``patch_vo_only_qwen_attention`` instead
 rotates the value projection and keeps the output projection — the weights the
 adapter runs with are the same.
+
+With a ``QwenTorquePagedCacheHIP`` the same adapter serves a batch: keys and
+values of every chunk, prompt or single tokens, are held once, in 8-bit pages
+(``ops.paged_append``, which also turns keys and queries to their positions and
+into the rotated basis), and every chunk attends to them
+(``ops.paged_attention``).
 """
 
 from __future__ import annotations
@@ -39,6 +45,7 @@ from torque_hip import _lib
 from torque_hip._tensors import stream_handle
 from torque_hip.cache_hip import TorqueKVCacheHIP
 from torque_hip.config import TorqueConfig
+from torque_hip.paged_cache import TorquePagedKVCache
 from torque_hip.quantization import Codebook
 from torque_hip.rotation import RotationSpec
 
@@ -218,6 +225,56 @@ def build_qwen_torque_cache(
     )
 
 
+@dataclass
+class QwenTorquePagedCacheHIP:
+    """One layer's cache of a batch: row b of every chunk belongs to ``sequences[b]`` of ``paged``."""
+
+    paged: TorquePagedKVCache
+    sequences: list[int]
+
+    @property
+    def rotation(self) -> RotationSpec | None:
+        return self.paged.rotation
+
+    @property
+    def offset(self) -> int:
+        return max((self.paged.length(s) for s in self.sequences), default=0)
+
+    def append_and_attend(self, queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, *, scale: float,
+                          cos: torch.Tensor | None = None, sin: torch.Tensor | None = None) -> torch.Tensor:
+        """A chunk's [B, H, L, D] queries, keys and values -> [B * L, Hq, D] attention output in the rotated basis.
+        ``cos`` / ``sin`` [B or 1, L, rotary_dim] turn queries and keys; None: they are turned already."""
+        batch, _, length, _ = queries.shape
+        if batch != len(self.sequences):
+            raise ValueError(f"the cache holds a batch of {len(self.sequences)}, got {batch}")
+        q, k, v = (x.transpose(1, 2).reshape(batch * length, x.shape[1], x.shape[3]) for x in (queries, keys, values))
+        tables: dict[str, Any] = {}
+        if cos is not None and sin is not None:
+            flat = [t.expand(batch, -1, -1).reshape(batch * length, t.shape[-1]) for t in (cos, sin)]
+            tables = dict(cos=flat[0], sin=flat[1], tables_by_token=True)
+        counts = [length] * batch
+        q = self.paged.append(k, v, query=q, sequences=self.sequences, counts=counts, **tables)
+        return self.paged.attend(q, sequences=self.sequences, counts=counts, scale=scale)
+
+
+def build_qwen_paged_cache(
+    *,
+    head_dim: int,
+    kv_heads: int,
+    batch: int,
+    max_tokens: int,
+    page_size: int = 64,
+    num_pages: int | None = None,
+    rotation_seed: int = 0,
+) -> QwenTorquePagedCacheHIP:
+    """One layer's paged cache with the adapter's settings: keys rotated on append, values not (the value projection is
+    pre-rotated); pages for ``max_tokens`` of each sequence unless ``num_pages`` is given."""
+    pages = batch * -(-max_tokens // page_size) if num_pages is None else num_pages
+    paged = TorquePagedKVCache(kv_heads=kv_heads, head_dim=head_dim, num_pages=pages, max_sequences=batch, max_tokens=max_tokens,
+                               page_size=page_size, rotation=RotationSpec.from_seed(head_dim, rotation_seed))
+    return QwenTorquePagedCacheHIP(paged=paged, sequences=[paged.add_sequence() for _ in range(batch)])
+
+
 # ---------------------------------------------------------------- attention adapter
 
 
@@ -323,11 +380,11 @@ def _dense_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale
     return F.scaled_dot_product_attention(q.to(torch.float32), k, v, attn_mask=cols <= rows, scale=scale)
 
 
-def _check_same_rotation(cache: QwenTorqueFullAttentionCacheHIP, rotation: RotationSpec) -> None:
+def _check_same_rotation(cache: QwenTorqueFullAttentionCacheHIP | QwenTorquePagedCacheHIP, rotation: RotationSpec) -> None:
     # The cache rotates keys and queries with its own signs; the adapter rotates the output back (and the
     # value projection was rotated) with ``rotation``: both must be the same transform.
-    own = cache.torque_cache.rotation
-    if not (np.array_equal(own.signs_left, rotation.signs_left) and np.array_equal(own.signs_right, rotation.signs_right)):
+    own = cache.rotation if isinstance(cache, QwenTorquePagedCacheHIP) else cache.torque_cache.rotation
+    if own is None or not (np.array_equal(own.signs_left, rotation.signs_left) and np.array_equal(own.signs_right, rotation.signs_right)):
         raise ValueError("the cache's rotation differs from the adapter's rotation")
 
 
@@ -337,11 +394,12 @@ class TorqueQwenAttention(torch.nn.Module):
 
     ``forward(hidden_states, position_embeddings, attention_mask=None, past_key_values=None)`` returns
     ``(output, None)`` like the wrapped module.  The cache is ``past_key_values`` when that is a
-    ``QwenTorqueFullAttentionCacheHIP``, else ``self.cache``; with no cache it is plain dense attention.
+    ``QwenTorqueFullAttentionCacheHIP`` or a ``QwenTorquePagedCacheHIP``, else ``self.cache``; with no cache it is plain
+    dense attention.  The paged cache takes batches; every row of a batch is as long as the others.
     """
 
     def __init__(self, base_attn: torch.nn.Module, *, rotation: RotationSpec,
-                 cache: QwenTorqueFullAttentionCacheHIP | None = None,
+                 cache: QwenTorqueFullAttentionCacheHIP | QwenTorquePagedCacheHIP | None = None,
                  rotary: Callable[..., tuple[torch.Tensor, torch.Tensor]] = apply_rotary) -> None:
         super().__init__()
         self.base_attn = base_attn
@@ -359,7 +417,11 @@ class TorqueQwenAttention(torch.nn.Module):
                 attention_mask: Any = None, past_key_values: Any = None, **kwargs: Any) -> tuple[torch.Tensor, None]:
         attn = self.base_attn
         B, L, _ = hidden_states.shape
-        if B != 1:
+        cache = self.cache
+        if isinstance(past_key_values, (QwenTorqueFullAttentionCacheHIP, QwenTorquePagedCacheHIP)):
+            cache = past_key_values
+            _check_same_rotation(cache, self.rotation)
+        if B != 1 and not isinstance(cache, QwenTorquePagedCacheHIP):
             raise ValueError("Torque HIP Qwen runtime currently supports batch size 1")
         hd = self.head_dim
         queries, gate = torch.chunk(attn.q_proj(hidden_states).view(B, L, -1, hd * 2), 2, dim=-1)
@@ -367,12 +429,16 @@ class TorqueQwenAttention(torch.nn.Module):
         keys = attn.k_norm(attn.k_proj(hidden_states).view(B, L, -1, hd)).transpose(1, 2)
         values = attn.v_proj(hidden_states).view(B, L, -1, hd).transpose(1, 2)
         cos, sin = position_embeddings
+        if isinstance(cache, QwenTorquePagedCacheHIP):
+            tables = dict(cos=cos, sin=sin)
+            if self.rotary is not apply_rotary:  # a rotary of the caller's own
+                queries, keys = self.rotary(queries, keys, cos, sin)
+                tables = {}
+            attended = cache.append_and_attend(queries, keys, values, scale=self.scaling, **tables)
+            output = attended.float().transpose(0, 1)[None]  # [1, Hq, B * L, D]
+            projected = _unrotate_gate(output, gate.reshape(1, B * L, -1, hd), rotation=self.rotation, dtype=attn.o_proj.weight.dtype)
+            return attn.o_proj(projected.reshape(B, L, -1)), None
         queries, keys = self.rotary(queries, keys, cos, sin)
-
-        cache = self.cache
-        if isinstance(past_key_values, QwenTorqueFullAttentionCacheHIP):
-            cache = past_key_values
-            _check_same_rotation(cache, self.rotation)
         if cache is not None and L == 1:
             output = cache.decode_token_and_append(queries.float(), keys.float(), values.float())
         elif cache is not None:
@@ -389,7 +455,8 @@ class TorqueQwenAttention(torch.nn.Module):
 
 @torch.no_grad()
 def patch_vo_only_qwen_attention(layer: torch.nn.Module, *, rotation: RotationSpec,
-                                 cache: QwenTorqueFullAttentionCacheHIP | None = None) -> TorqueQwenAttention:
+                                 cache: QwenTorqueFullAttentionCacheHIP | QwenTorquePagedCacheHIP | None = None
+                                 ) -> TorqueQwenAttention:
     """Replace ``layer.self_attn`` (a module with the reference model's original weights) by the adapter.
 
     The value projection's head blocks (weight and bias) are multiplied by the rotation in place, as the
