@@ -46,7 +46,7 @@ PagedPlan plan_attention(int64_t tokens, int batch, bool ragged, int group, int 
   p.items = ragged ? tokens * group / p.rows + batch : static_cast<int64_t>(batch) * ((group + p.rows - 1) / p.rows);
   const int64_t tiles = (static_cast<int64_t>(max_pages) * page_size + kTile - 1) / kTile;  // of one sequence, at most
   const int64_t units = p.items * kv_heads;
-  if (tiles <= kLeastTiles || units >= (p.chunk ? 1 : 16) * static_cast<int64_t>(num_cus)) return p;
+  if (tiles <= kLeastTiles || units >= (p.chunk ? 1 : 16) * static_cast<int64_t>(num_cus) || p.items * tiles >= INT_MAX) return p;
   const int64_t fill = std::max<int64_t>(1, (p.chunk ? (head_dim == 256 ? 1 : 2) : 1) * static_cast<int64_t>(num_cus) / kv_heads);
   const int64_t most = std::max<int64_t>(1, (p.items * tiles + kLeastTiles - 1) / kLeastTiles);
   p.workgroups = static_cast<int>(std::min(fill, most));

@@ -50,21 +50,24 @@ struct PagedItem {
   int tiles;       // tiles of keys that its last token sees
 };
 
+// Counts of rows (tokens x group), items and tiles of a call stay below 2^31 (the
+// host sees to it), so that nothing here divides 64 bits.
 template <int R>
-__device__ __forceinline__ int64_t paged_item_base(const PagedAttentionArgs& a, int b) {
-  if (a.batch.starts == nullptr) return static_cast<int64_t>(b) * ((a.group + R - 1) / R);
-  return static_cast<int64_t>(paged_start(a.batch, b)) * a.group / R + b;
+__device__ __forceinline__ int paged_item_base(const PagedAttentionArgs& a, int b) {
+  if (a.batch.starts == nullptr) return b * ((a.group + R - 1) / R);
+  return paged_start(a.batch, b) * a.group / R + b;
 }
 
 template <int R>
-__device__ __forceinline__ PagedItem paged_item_of(const PagedAttentionArgs& a, int b, int64_t unit) {
+__device__ __forceinline__ PagedItem paged_item_of(const PagedAttentionArgs& a, int b, int unit) {
   PagedItem it;
   it.b = b;
   it.s = paged_sequence(a.batch, b);
-  const int64_t all = static_cast<int64_t>(it.s.rows) * a.group, row0 = unit * R;
-  it.rows = unit < 0 ? 0 : static_cast<int>(min(max(all - row0, int64_t(0)), int64_t(R)));
-  it.row0 = static_cast<int>(row0);
-  const int64_t last = it.rows == 0 ? 0 : (row0 + it.rows - 1) / a.group;
+  const int all = it.s.rows * a.group;
+  const bool some = unit >= 0 && unit <= all / R;
+  it.row0 = some ? unit * R : 0;
+  it.rows = some ? min(all - it.row0, R) : 0;
+  const int last = it.rows == 0 ? 0 : (it.row0 + it.rows - 1) / a.group;
   const int64_t keys = min(max(it.s.first + last + 1, int64_t(0)), static_cast<int64_t>(it.s.len));
   it.tiles = static_cast<int>((keys + kTile - 1) / kTile);
   return it;
@@ -92,10 +95,9 @@ __device__ __forceinline__ PagedItem paged_item(const PagedAttentionArgs& a, int
 // sees nothing, so that somebody writes its zeros.
 __device__ __forceinline__ int paged_cost(const PagedItem& it) { return it.rows == 0 ? 0 : max(it.tiles, 1); }
 
-// Sum of the lanes up to and with this one.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
+// Sum of the lanes up to and with this one, of the first `lanes`.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, int lanes) {
+  for (int d = 1; d < lanes; d <<= 1) {
     const uint32_t other = static_cast<uint32_t>(__shfl_up(static_cast<int>(v), d));
     if (lane_id() >= d) v += other;
   }
@@ -122,46 +124,47 @@ __device__ __forceinline__ void paged_schedule(const PagedAttentionArgs& a, int 
     const PagedItem it = paged_item<R>(a, index);
     if (it.rows > 0) work(it, 0, it.tiles, true, 0);
   } else {
-    const int workgroups = gridDim.x, lane = lane_id();
+    const uint32_t workgroups = gridDim.x;
+    const int lane = lane_id();
     auto cost_of = [&](int index) { return index < a.items ? static_cast<uint32_t>(paged_cost(paged_item<R>(a, index))) : 0u; };
-    uint32_t mine = cost_of(lane), sum = wave_scan(mine);
-    int64_t total = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum), 63));
+    auto lanes_of = [&](int i0) { return min(a.items - i0, kWave); };
+    auto lane_of = [](uint32_t v, int k) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), k)); };
+    uint32_t mine = cost_of(lane), sum = wave_scan(mine, lanes_of(0));
+    uint32_t total = lane_of(sum, lanes_of(0) - 1);
     for (int i0 = kWave; i0 < a.items; i0 += kWave)
-      total += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan(cost_of(i0 + lane))), 63));
-    const int64_t run = max((total + workgroups - 1) / workgroups, static_cast<int64_t>(a.least_tiles));
-    int64_t at = run * blockIdx.x;
-    const int64_t end = min(at + run, total);
+      total += lane_of(wave_scan(cost_of(i0 + lane), lanes_of(i0)), lanes_of(i0) - 1);
+    const uint32_t run = max((total + workgroups - 1) / workgroups, static_cast<uint32_t>(a.least_tiles));
+    uint32_t at = run * blockIdx.x;  // below 2^32: a run more than the total at most, and least_tiles for each workgroup
+    const uint32_t end = min(at + run, total);
     if (at >= end) return;
     int index = a.items;  // nothing to do, were no item found
-    int64_t offset = 0, base = 0;
+    uint32_t offset = 0, base = 0;
     for (int i0 = 0; i0 < a.items; i0 += kWave) {
       if (i0 > 0) {
         mine = cost_of(i0 + lane);
-        sum = wave_scan(mine);
+        sum = wave_scan(mine, lanes_of(i0));
       }
-      const uint32_t all = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum), 63));
+      const uint32_t all = lane_of(sum, lanes_of(i0) - 1);
       if (at < base + all) {  // the item that holds tile `at`: the first whose sum passes it
-        const int k = __ffsll(__ballot(base + sum > at)) - 1;
+        const int k = __ffsll(__ballot(lane < lanes_of(i0) && base + sum > at)) - 1;
         index = i0 + k;
-        offset = at - base - static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum - mine), k));
+        offset = at - base - lane_of(sum - mine, k);
         break;
       }
       base += all;
     }
     while (at < end && index < a.items) {
       const PagedItem it = paged_item<R>(a, index);
-      const int cost = paged_cost(it);
+      const uint32_t cost = paged_cost(it);
       if (cost > 0) {
-        const int64_t take = min(cost - offset, end - at);
+        const uint32_t take = min(cost - offset, end - at);
         if (offset == 0 && threadIdx.x == 0) {
-          const int64_t first = at / run, last = (at + cost - 1) / run;
+          const uint32_t last = (at + cost - 1) / run;  // at / run is this workgroup
           a.cut[static_cast<int64_t>(index) * a.batch.kv_heads + h] =
-              make_int2(static_cast<int>(first), last > first ? static_cast<int>(last - first + 1) : 0);
+              make_int2(static_cast<int>(blockIdx.x), last > blockIdx.x ? static_cast<int>(last - blockIdx.x + 1) : 0);
         }
-        const bool whole = take == cost;
-        const int from = static_cast<int>(min(offset, static_cast<int64_t>(it.tiles)));
-        const int to = static_cast<int>(min(offset + take, static_cast<int64_t>(it.tiles)));
-        work(it, from, to, whole, offset == 0 ? 1 : 0);
+        const int from = min(static_cast<int>(offset), it.tiles), to = min(static_cast<int>(offset + take), it.tiles);
+        work(it, from, to, take == cost, offset == 0 ? 1 : 0);
         at += take;
       }
       offset = 0;
@@ -274,10 +277,10 @@ __device__ __forceinline__ float paged_unit(uint32_t top, float* f) {
 //
 // A wavefront's next keys are on their way from the moment the current ones are
 // multiplied, its next values likewise, and page numbers a tile before that.
-constexpr int split_waves(int d) { return d == 256 ? 4 : 8; }
+constexpr int split_waves(int d) { return d == 256 ? 4 : d == 128 ? 8 : 12; }
 
 template <int D, int PLANES, bool CUT>
-__global__ __launch_bounds__(split_waves(D) * kWave, (D == 256 ? 1 : 2)) void paged_split_kernel(const PagedAttentionArgs a) {
+__global__ __launch_bounds__(split_waves(D) * kWave, split_waves(D) / 4) void paged_split_kernel(const PagedAttentionArgs a) {
   constexpr int R = 16, C = D / 64, DT = D / 16, kSplitWaves = split_waves(D);
   constexpr int P = D + 4;  // LDS pitch of a row of sums
   constexpr float kUnit = PLANES == 3 ? 8323072.f : 32512.f;  // 127 x 256^(PLANES-1)
@@ -291,9 +294,11 @@ __global__ __launch_bounds__(split_waves(D) * kWave, (D == 256 ? 1 : 2)) void pa
 
   paged_schedule<R, CUT>(a, h, [&](const PagedItem& it, int from, int to, bool whole, int slot) {
     // ---- page numbers: this lane's key rows are in group j / 4 of a tile's 16 tokens, its values and scores in group g
-    auto page_of = [&](int tile, int group) {
-      const int64_t t = static_cast<int64_t>(tile) * kTile + 16 * group;
-      return tile < to && t < it.s.len ? paged_page(p, it.b, t >> p.log_page) : -1;
+    const int32_t* list = p.table + it.b * p.table_stride;
+    auto page_of = [&](int tile, int group) {  // a length is at most what the list holds
+      const int t = tile * kTile + 16 * group;
+      const int id = tile < to && t < it.s.len ? list[t >> p.log_page] : -1;
+      return id < p.num_pages ? id : -1;  // below 0: none either
     };
     PagedI4 kv[4][C], vv[DT];
     float ks, vs;
@@ -386,10 +391,15 @@ __global__ __launch_bounds__(split_waves(D) * kWave, (D == 256 ? 1 : 2)) void pa
         for (int r = 0; r < 4; ++r) {
           float f = static_cast<float>(hi[r]);
           if constexpr (PLANES == 3) f = fmaf(f, 256.f, static_cast<float>(lo[r]));
-          w[4 * s + r] = 4 * s + r < seen ? fmaf(f, by, shift) : -INFINITY;
-          top = fmaxf(top, w[4 * s + r]);
+          w[4 * s + r] = fmaf(f, by, shift);
         }
       }
+      if (__ballot(seen < 16) != 0) {  // a sequence's last tile, an earlier draft, a page that is none
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = i < seen ? w[i] : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, w[i]);
       if (tile + kSplitWaves < to) {
         load_keys(tile + kSplitWaves, knext);
         load_scales(vnext);
@@ -405,10 +415,19 @@ __global__ __launch_bounds__(split_waves(D) * kWave, (D == 256 ? 1 : 2)) void pa
         sum += e;
         n[i] = __float_as_uint(fmaf(e, kUnit, kMagic));  // the integer in the mantissa's low bits
       }
-      const float next = fmaxf(m, top);
-      const float keep = m == next ? 1.f : fast_exp2(m - next), part = top == -INFINITY ? 0.f : fast_exp2(top - next);
-      l = l * keep + (vid >= 0 ? sum * part * back : 0.f);
-      m = next;
+      // The running maximum moves where a tile exceeds it by 2^8 and more, in few tiles: sums are multiplied then only.
+      if (__ballot(top > m + 8.f) != 0) {
+        const float next = fmaxf(m, top);
+        const float keep = m == next ? 1.f : fast_exp2(m - next);
+        m = next;
+        l *= keep;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[t][r] *= keep;
+      }
+      const float part = top == -INFINITY ? 0.f : fast_exp2(top - m);
+      l = fmaf(sum, vid >= 0 ? part * back : 0.f, l);
 
       PagedI4 wq[PLANES];
 #pragma unroll
@@ -430,7 +449,7 @@ __global__ __launch_bounds__(split_waves(D) * kWave, (D == 256 ? 1 : 2)) void pa
         for (int r = 0; r < 4; ++r) {
           float f = static_cast<float>(hi[r]);
           if constexpr (PLANES == 3) f = fmaf(f, 256.f, static_cast<float>(lo[r]));
-          acc[t][r] = fmaf(f, part, acc[t][r] * keep);
+          acc[t][r] = fmaf(f, part, acc[t][r]);
         }
       }
       if (tile + kSplitWaves < to) load_values(tile + kSplitWaves, vnext);
@@ -493,17 +512,17 @@ __global__ __launch_bounds__(kBlock) void paged_merge_kernel(const PagedAttentio
   __shared__ float s_sum[kWavesPerBlock][D + 2];
   const PagedBatch& p = a.batch;
   const int heads = p.kv_heads * a.group, wave = threadIdx.x >> 6, lane = lane_id();
-  const int64_t row = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave : blockIdx.x;
-  if (row >= static_cast<int64_t>(p.tokens) * heads) return;
-  const int token = static_cast<int>(row / heads), head = static_cast<int>(row - static_cast<int64_t>(token) * heads);
+  const uint32_t row = WAVES == 1 ? blockIdx.x * kWavesPerBlock + wave : blockIdx.x;
+  if (row >= static_cast<uint32_t>(p.tokens) * heads) return;
+  const int token = row / heads, head = row - token * heads;
   const int h = head / a.group;
   int b = token;
   if (p.starts != nullptr) b = wave_last(p.batch, token, [&](int i) { return static_cast<int64_t>(paged_start(p, i)); });
   const PagedSequence s = paged_sequence(p, b);
   if (token < s.row0 || token >= s.row0 + s.rows) return;
-  const int64_t local = static_cast<int64_t>(token - s.row0) * a.group + head - h * a.group;
+  const int local = (token - s.row0) * a.group + head - h * a.group;
   const int64_t item = paged_item_base<R>(a, b) + local / R;
-  const int r = static_cast<int>(local % R);
+  const int r = local % R;
   const int2 cut = a.cut[item * p.kv_heads + h];
   if (cut.x < 0 || cut.y <= 0 || cut.y > a.workgroups - cut.x) return;  // whole, or (row offsets that decrease) not dealt out
   auto slot = [&](int k) { return ((static_cast<int64_t>(cut.x + k) * p.kv_heads + h) * 2 + (k == 0 ? 1 : 0)) * R + r; };

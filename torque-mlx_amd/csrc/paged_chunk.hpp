@@ -143,10 +143,9 @@ struct DigitScores {
 
 // paged_chunk_kernel<D, TERMS>: 128 rows to a workgroup, 32 to a wavefront; the
 // wavefronts share each tile of 64 keys through LDS.  At head_dim 256 a second
-// four wavefronts take the same rows and the other half of the value dimensions:
-// the scores are computed twice, but a wavefront's sums fit its registers beside
-// the query, so that two run on a SIMD and one's products cover the other's
-// exponentials.
+// four wavefronts take the same rows: either four score half of a tile's keys and
+// sum half of the value dimensions, the weights going through LDS between, so that
+// a wavefront's sums fit its registers beside the query and two run on a SIMD.
 //
 // The weights are rounded to float16, 2^-12 of themselves at most, an error of the
 // size of a 16-bit result's own; for float32 queries (TERMS 2) a second product
@@ -165,7 +164,7 @@ template <int D, int TERMS, bool CUT>
 __global__ __launch_bounds__(chunk_threads(D), 2) void paged_chunk_kernel(const PagedAttentionArgs a) {
   using Scores = std::conditional_t<D == 256, DigitScores<D, TERMS>, HalfScores<D, TERMS>>;
   constexpr int NT = chunk_threads(D), R = kChunkRows, HALVES = NT / 256;
-  constexpr int DH = D / HALVES, DT = DH / 32;
+  constexpr int DH = D / HALVES, DT = DH / 32, SUBS = 2 / HALVES;  // halves of a tile that a wavefront scores
   constexpr int KP = Scores::kPitch, VP = kTile + 8;  // LDS pitches: bytes of a key, float16 of a value dimension
   constexpr int UNITS = 4 * D / NT;                   // 16-byte pieces of a tile's keys (values) to a thread
   constexpr float kLift = 7.f;
@@ -175,6 +174,9 @@ __global__ __launch_bounds__(chunk_threads(D), 2) void paged_chunk_kernel(const 
   // key scales, log2 of the value scales and their inverses (0: no page)
   __shared__ __align__(16) int s_next[2][4];
   __shared__ __align__(16) float s_scale[2][3][4];
+  // HALVES 2: the rows' maxima over either half of a tile, and the weights of a tile
+  __shared__ float s_top[HALVES][HALVES == 2 ? R : 1];
+  __shared__ __align__(16) PagedH8 s_w[HALVES == 2 ? 4 : 1][4][TERMS][kWave];
   const PagedBatch& p = a.batch;
   const int tid = threadIdx.x, lane = lane_id(), wave = tid >> 6;
   const int j = lane & 31, g = lane >> 5;
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(chunk_threads(D), 2) void paged_chunk_kernel(const 
   const int T = 1 << p.log_page;
 
   paged_schedule<R, CUT>(a, h, [&](const PagedItem& it, int from, int to, bool whole, int slot) {
-    const int r0 = 32 * (wave & 3), d0 = DH * (wave >> 2);
+    const int half = wave >> 2, r0 = 32 * (wave & 3), d0 = DH * half;
     const bool live = r0 + j < it.rows;
     const PagedRowAt at = paged_row(a, it, h, live ? r0 + j : 0);
     const int64_t keys = live ? at.keys : 0;
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(chunk_threads(D), 2) void paged_chunk_kernel(const 
     for (int tile = from; tile < to; ++tile) {
       const int buffer = (tile - from) & 1;
       put(buffer);
-      __syncthreads();
+      lds_barrier();
       if (tile + 1 < to) {
         fetch(*reinterpret_cast<const int4*>(s_next[buffer]), tile + 1);
         if (tid < 4) {
@@ -265,35 +267,42 @@ __global__ __launch_bounds__(chunk_threads(D), 2) void paged_chunk_kernel(const 
         }
       }
       const int64_t tok0 = static_cast<int64_t>(tile) * kTile;
-      if (tok0 < some_see) {
+      if (HALVES == 2 || tok0 < some_see) {
         const float4 k4 = *reinterpret_cast<const float4*>(s_scale[buffer][0]), s4 = *reinterpret_cast<const float4*>(s_scale[buffer][1]);
         const float4 b4 = *reinterpret_cast<const float4*>(s_scale[buffer][2]);
         const float ks[4] = {k4.x, k4.y, k4.z, k4.w}, shift[4] = {s4.x, s4.y, s4.z, s4.w}, back[4] = {b4.x, b4.y, b4.z, b4.w};
         const bool here = tok0 + kTile <= all_see && b4.x != 0.f && b4.y != 0.f && b4.z != 0.f && b4.w != 0.f;
-        float w[2][16];
+        float w[SUBS][16];
         float top = -INFINITY;
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int n = 0; n < SUBS; ++n) {
+          const int s = HALVES == 2 ? half : n;
           // row i of the product is token 16 (i / 16) + 8 (i / 4 mod 2) + 4 (i / 8 mod 2) + i mod 4
           const int row = 32 * s + 16 * (j >> 4) + 8 * ((j >> 2) & 1) + 4 * ((j >> 3) & 1) + (j & 3);
-          scores.run(s_k[buffer], row, g, w[s]);
+          scores.run(s_k[buffer], row, g, w[n]);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int group = 2 * s + (r >> 3);
-            w[s][r] = fmaf(w[s][r], ks[group] * unit, shift[group]);
+            const float by = s == 0 ? (r < 8 ? ks[0] : ks[1]) : (r < 8 ? ks[2] : ks[3]);
+            const float up = s == 0 ? (r < 8 ? shift[0] : shift[1]) : (r < 8 ? shift[2] : shift[3]);
+            w[n][r] = fmaf(w[n][r], by * unit, up);
           }
           if (!here) {
+            const int64_t left = keys - (tok0 + 32 * s + 8 * g);  // keys seen from this lane's first on
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const int group = 2 * s + (r >> 3);
-              const int64_t token = tok0 + 32 * s + 16 * (r >> 3) + 8 * g + (r & 7);
-              w[s][r] = back[group] != 0.f && token < keys ? w[s][r] : -INFINITY;
+              const float b = s == 0 ? (r < 8 ? back[0] : back[1]) : (r < 8 ? back[2] : back[3]);
+              w[n][r] = b != 0.f && 16 * (r >> 3) + (r & 7) < left ? w[n][r] : -INFINITY;
             }
           }
 #pragma unroll
-          for (int r = 0; r < 16; ++r) top = fmaxf(top, w[s][r]);
+          for (int r = 0; r < 16; ++r) top = fmaxf(top, w[n][r]);
         }
         top = xor_reduce<32, OpMax>(top);
+        if constexpr (HALVES == 2) {  // the other half's maximum: both halves' weights are relative to the same
+          if (g == 0) s_top[half][r0 + j] = top;
+          lds_barrier();
+          top = fmaxf(top, s_top[1 - half][r0 + j]);
+        }
         if (__ballot(top > m + 8.f) != 0) {
           const float next = fmaxf(m, top);
           const float keep = m == next ? 1.f : fast_exp2(m - next);
@@ -303,32 +312,60 @@ __global__ __launch_bounds__(chunk_threads(D), 2) void paged_chunk_kernel(const 
           for (int t = 0; t < DT; ++t) acc[t] *= keep;
         }
         const float base = m == -INFINITY ? 0.f : m - kLift;
-#pragma unroll
-        for (int kc = 0; kc < 4; ++kc) {  // 16 tokens, one page
-          float e[8], sum = 0.f;
-          PagedH8 ph, pl;
+        auto weigh = [&](const float* x, PagedH8* p16) {  // of 16 tokens, one page; their sum
+          float sum = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            e[i] = fast_exp2(w[kc >> 1][8 * (kc & 1) + i] - base);
-            sum += e[i];
+            const float e = fast_exp2(x[i] - base);
+            sum += e;
+            p16[0][i] = static_cast<_Float16>(e);
+            if constexpr (TERMS == 2) p16[TERMS - 1][i] = static_cast<_Float16>(e - static_cast<float>(p16[0][i]));
           }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            ph[i] = static_cast<_Float16>(e[i]);
-            if constexpr (TERMS == 2) pl[i] = static_cast<_Float16>(e[i] - static_cast<float>(ph[i]));
-          }
-          l = fmaf(sum, back[kc], l);
+          return sum;
+        };
+        auto gather = [&](int kc, const PagedH8* p16) {
 #pragma unroll
           for (int t = 0; t < DT; ++t) {
             const PagedH8 v = *reinterpret_cast<const PagedH8*>(s_v[buffer] + (d0 + 32 * t + j) * VP + 16 * kc + 8 * g);
-            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, acc[t], 0, 0, 0);
-            if constexpr (TERMS == 2) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, acc[t], 0, 0, 0);
+#pragma unroll
+            for (int n = 0; n < TERMS; ++n) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p16[n], acc[t], 0, 0, 0);
+          }
+        };
+        if constexpr (HALVES == 2) {
+          PagedH8 own[2][TERMS];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const float sum = weigh(w[0] + 8 * n, own[n]);
+            l = fmaf(sum, half == 0 ? (n == 0 ? back[0] : back[1]) : (n == 0 ? back[2] : back[3]), l);
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) s_w[wave & 3][2 * half + n][k][lane] = own[n][k];
+          }
+          lds_barrier();
+#pragma unroll
+          for (int kc = 0; kc < 4; ++kc) {
+            PagedH8 p16[TERMS];
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) p16[k] = s_w[wave & 3][kc][k][lane];
+            gather(kc, p16);
+          }
+        } else {
+#pragma unroll
+          for (int kc = 0; kc < 4; ++kc) {
+            PagedH8 p16[TERMS];
+            l = fmaf(weigh(w[kc >> 1] + 8 * (kc & 1), p16), back[kc], l);
+            gather(kc, p16);
           }
         }
       }
     }
 
     l = xor_reduce<32, OpSum>(l);
+    if constexpr (HALVES == 2) {  // either half has summed its own tokens' weights
+      __syncthreads();
+      if (g == 0) s_top[half][r0 + j] = l;
+      __syncthreads();
+      l += s_top[1 - half][r0 + j];
+    }
     if (!live) return;
     if (whole) {
       const int64_t o = at.token * a.o_token_stride + at.head * a.o_head_stride + d0 + 4 * g;
