@@ -415,6 +415,12 @@ int tq_paged_dequantize(const int32_t* page_ids, int64_t count, const int8_t* ke
 size_t tq_paged_attention_workspace_bytes(int64_t tokens, int batch, int ragged, int query_heads, int kv_heads,
                                           int head_dim, int max_pages, int page_size, int64_t max_tokens, int num_cus);
 
+/* The name of the attention kernel such a call launches, e.g.
+ * "paged_split_kernel<128>" (few rows) or "paged_chunk_kernel<128>" (many); NULL
+ * for bad arguments (see tq_last_error). */
+const char* tq_paged_attention_kernel(int64_t tokens, int batch, int ragged, int query_heads, int kv_heads,
+                                      int head_dim, int max_pages, int page_size, int64_t max_tokens, int num_cus);
+
 /* Causal attention of each sequence's newest tokens over its pages: row i of n
  * stands at position context_lens[b] - n + i and sees the keys up to it;
  * a row that sees none gives zeros.  out has the query's dtype; rows of no

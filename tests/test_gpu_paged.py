@@ -8,7 +8,7 @@ import paged_model as model
 import pytest
 import torch
 
-from torque_hip import ops
+from torque_hip import _lib, ops
 
 pytestmark = pytest.mark.gpu
 TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
@@ -63,6 +63,62 @@ def test_attention_against_64_bits(hip_device, dim, size, dtype, kv, group, news
     if starts is None:  # the same rows, named by their offsets
         same = ops.paged_attention(query, page_table=pool.table, context_lens=pool.lens, token_starts=starts_of(news), **pool.t)
         check_attention(pool, query, news, lens, same)
+
+
+CHUNKS = [
+    # dim, page, dtype, kv, group, tokens each sequence adds, lengths with them
+    (128, 64, "bf16", 1, 4, [70, 0, 33], [70, 10, 300]),
+    (256, 32, "bf16", 1, 2, [130], [400]),
+    (256, 16, "f32", 2, 3, [45, 22], [45, 500]),
+    (64, 16, "f32", 2, 1, [200], [777]),
+    (128, 32, "f16", 2, 4, [257, 64], [257, 1000]),
+    (128, 16, "f32", 1, 5, [31, 2, 100], [200, 2, 163]),
+    (64, 64, "f16", 3, 7, [64], [65]),
+    (256, 64, "f16", 1, 17, [9, 40], [9, 700]),
+]
+
+
+@pytest.mark.parametrize("dim,size,dtype,kv,group,news,lens", CHUNKS)
+def test_chunks_against_64_bits(hip_device, dim, size, dtype, kv, group, news, lens):
+    """The kernel for many rows, which a table wide enough for long sequences chooses: other pages behind the end, a page
+    that is none, rows of no sequence and an output with strides."""
+    pool = model.Pool(lens, kv=kv, dim=dim, size=size, seed=3, width=400_000 // size).fill()
+    n = sum(news)
+    shape = (n + 3, len(news), 1, kv * group, kv, dim, pool.table.shape[1], size, max(news), 0)
+    assert _lib.call("tq_paged_attention_kernel", *shape) == b"paged_chunk_kernel<%d>" % dim
+    query = randn(5, n + 3, kv * group, dim, dtype=TYPES[dtype])
+    kw = dict(page_table=pool.table, context_lens=pool.lens, token_starts=starts_of(news), max_tokens=max(news), **pool.t)
+    large = torch.full((kv * group, n + 3, dim + 8), 5.0, dtype=TYPES[dtype], device="cuda")
+    out = ops.paged_attention(query, out=large.transpose(0, 1)[..., 4 : dim + 4], **kw)
+    check_attention(pool, query, news, lens, out)
+    assert bool((large[:, n:] == 5).all()) and bool((large[..., :4] == 5).all()) and bool((large[..., dim + 4 :] == 5).all())
+    again = ops.paged_attention(query, **kw)
+    assert torch.equal(again[:n], out[:n]) and bool((again[n:] == 0).all())
+    few = ops.paged_attention(query, **{**kw, "max_tokens": 1})  # a hint that is wrong chooses the other kernel, no more
+    check_attention(pool, query, news, lens, few)
+    b = len(news) - 1
+    pool.table[b, (lens[b] - 1) // size // 2] = -1
+    check_attention(pool, query, news, lens, ops.paged_attention(query, **kw))
+
+
+def test_chunks_of_many_sequences(hip_device):
+    """So many units of rows that each has a workgroup of its own, and bad queries among them."""
+    g = torch.Generator().manual_seed(1)
+    news = torch.randint(0, 40, (40,), generator=g).tolist()
+    news[3], news[7] = 70, 0
+    lens = [n + int(x) for n, x in zip(news, torch.randint(0, 90, (40,), generator=g))]
+    pool = model.Pool(lens, kv=8, dim=64, size=16, seed=3, width=8192).fill()
+    assert _lib.call("tq_paged_attention_kernel", sum(news), 40, 1, 8, 8, 64, 8192, 16, 70, 0) == b"paged_chunk_kernel<64>"
+    assert _lib.call("tq_paged_attention_workspace_bytes", sum(news), 40, 1, 8, 8, 64, 8192, 16, 70, 0) == 0  # nothing is cut
+    query = randn(5, sum(news), 8, 64, dtype=torch.bfloat16)
+    kw = dict(page_table=pool.table, context_lens=pool.lens, token_starts=starts_of(news), max_tokens=max(news), **pool.t)
+    out = ops.paged_attention(query, **kw)
+    check_attention(pool, query, news, lens, out)
+    query[5, 2, 7], query[100, 0, 0] = math.inf, math.nan
+    bad = ops.paged_attention(query, **kw)
+    assert bool(bad[5, 2].isnan().all()) and bool(bad[100, 0].isnan().all())
+    bad[5, 2], bad[100, 0] = out[5, 2], out[100, 0]
+    assert torch.equal(bad, out)
 
 
 def test_rows_that_see_nothing_are_zero(hip_device):
@@ -164,11 +220,11 @@ def test_scale_and_bad_queries(hip_device):
 
 
 @pytest.mark.parametrize("spread", [0, 30])
-@pytest.mark.parametrize("new", [1, 100])
-def test_scales_far_apart(hip_device, spread, new):
+@pytest.mark.parametrize("new,width", [(1, 32), (100, 32), (100, 4096)])
+def test_scales_far_apart(hip_device, spread, new, width):
     """Pages whose scales differ by up to 2^30, one sharp row among them."""
     lens = [500]
-    pool = model.Pool(lens, kv=1, dim=64, size=16, seed=2).fill(spread=6)
+    pool = model.Pool(lens, kv=1, dim=64, size=16, seed=2, width=width).fill(spread=6)
     pool.t["value_scales"].mul_(torch.exp2(torch.randint(-spread, 1, pool.t["value_scales"].shape).float()).cuda())
     query = randn(6, new, 3, 64) * torch.tensor([0.01, 1.0, 8.0], device="cuda")[None, :, None]
     out = ops.paged_attention(query, page_table=pool.table, context_lens=pool.lens, token_starts=starts_of([new]), **pool.t)

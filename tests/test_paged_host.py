@@ -115,6 +115,17 @@ def test_workspace_bytes():
     assert ws(1, 1, 0, 30, 8, 128, 512, 64, 1) == 0 and ws(1, 1, 0, 8, 8, 100, 512, 64, 1) == 0  # refused shapes
 
 
+def test_kernel_choice():
+    name = lambda *a: _lib.call("tq_paged_attention_kernel", *a, 256)  # noqa: E731
+    assert name(1, 1, 0, 32, 8, 128, 2000, 64, 1) == b"paged_split_kernel<128>"
+    assert name(16, 1, 1, 32, 8, 128, 500, 64, 16) == b"paged_chunk_kernel<128>"  # half a unit of rows over 32000 keys
+    assert name(15, 1, 1, 32, 8, 128, 500, 64, 15) == b"paged_split_kernel<128>"
+    assert name(128, 1, 1, 32, 8, 128, 32, 64, 128) == b"paged_split_kernel<128>"  # 512 rows over 2000 keys
+    assert name(512, 1, 1, 32, 8, 128, 8, 64, 512) == b"paged_chunk_kernel<128>"  # enough units of rows
+    assert name(64, 64, 1, 32, 8, 128, 500, 64, 0) == b"paged_split_kernel<128>"  # the most rows unknown: as if even
+    assert name(1, 1, 0, 30, 8, 128, 10, 64, 1) is None and name(0, 1, 0, 8, 8, 128, 10, 64, 1) is None
+
+
 def pool(count=4, kv=2, size=16, dim=64):
     return dict(key_pages=torch.zeros(count, kv, size, dim, dtype=torch.int8), value_pages=torch.zeros(count, kv, dim, size, dtype=torch.int8),
                 key_scales=torch.ones(count, kv), value_scales=torch.ones(count, kv))

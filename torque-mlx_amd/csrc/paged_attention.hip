@@ -33,18 +33,34 @@ constexpr int kLeastTiles = 8;  // tiles of 64 keys that a workgroup takes at le
 
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
-// Rows (tokens x group) of a sequence from which the chunk kernel runs.
-constexpr int64_t kChunkFrom = 48;
+// Which kernel runs.  The chunk kernel reads a tile of keys once for 128 rows and
+// the split kernel once for 16, but a tile costs a chunk workgroup 2 to 3 us however
+// few of its rows are there, and fewer workgroups share the keys.  Measured, split /
+// chunk in us (16-bit queries, 8 heads of the cache; 4 at head_dim 256):
+//   head_dim 128, one sequence: 128 rows over 2000 keys 17.9 / 32.1, over 8000 33 /
+//   36, over 32000 65 / 50; 512 rows over 8000 64 / 58; 2048 rows over 512 31 / 28,
+//   over 2000 93 / 68
+//   eight sequences: 128 rows over 4000 58 / 57, 256 over 1000 72 / 60, 512 over 128 52 / 21
+//   head_dim 256: 64 rows over 32000 59 / 53, 512 over 8000 85 / 70, 2048 over 2000 104 / 77
+//   head_dim 64: 128 rows over 32000 40 / 39, 1024 over 8000 64 / 57
+// so a sequence has to bring half a unit of rows, and the call either enough units
+// or enough rows x tiles x heads.  Lengths lie on the device: the page table's
+// width stands for them, so a table wider than its sequences favours the chunk kernel.
+constexpr int64_t kChunkRowsLeast = kChunkRows / 2;
+constexpr int64_t kChunkUnits = 128;
+constexpr double kChunkWork = 1 << 18;
 
 PagedPlan plan_attention(int64_t tokens, int batch, bool ragged, int group, int kv_heads, int head_dim, int max_pages,
                          int page_size, int64_t max_tokens, int num_cus) {
   PagedPlan p{};
   if (!ragged) max_tokens = 1;
   if (max_tokens <= 0) max_tokens = (tokens + batch - 1) / batch;  // unknown: as if all had as many
-  p.chunk = std::min(max_tokens, tokens) * group >= kChunkFrom;
+  const int64_t tiles = (static_cast<int64_t>(max_pages) * page_size + kTile - 1) / kTile;  // of one sequence, at most
+  const int64_t rows = tokens * group;
+  p.chunk = std::min(max_tokens, tokens) * group >= kChunkRowsLeast &&
+            ((rows + kChunkRows - 1) / kChunkRows * kv_heads >= kChunkUnits || static_cast<double>(rows) * tiles * kv_heads >= kChunkWork);
   p.rows = p.chunk ? kChunkRows : kSplitRows;
   p.items = ragged ? tokens * group / p.rows + batch : static_cast<int64_t>(batch) * ((group + p.rows - 1) / p.rows);
-  const int64_t tiles = (static_cast<int64_t>(max_pages) * page_size + kTile - 1) / kTile;  // of one sequence, at most
   const int64_t units = p.items * kv_heads;
   if (tiles <= kLeastTiles || units >= (p.chunk ? 1 : 16) * static_cast<int64_t>(num_cus) || p.items * tiles >= INT_MAX) return p;
   const int64_t fill = std::max<int64_t>(1, (p.chunk ? (head_dim == 256 ? 1 : 2) : 1) * static_cast<int64_t>(num_cus) / kv_heads);
@@ -93,18 +109,44 @@ int launch_attention_d(const PagedAttentionArgs& a, const PagedPlan& plan, hipSt
   return a.query_type == TQ_F32 ? launch_planned<D, 3>(a, plan, stream) : launch_planned<D, 2>(a, plan, stream);
 }
 
+// A call's plan as the host queries ask for it.
+int plan_for(int64_t tokens, int batch, int ragged, int query_heads, int kv_heads, int head_dim, int max_pages, int page_size,
+             int64_t max_tokens, int num_cus, PagedPlan* p) {
+  int rc = check_pages(1, page_size, kv_heads, head_dim);
+  if (rc) return rc;
+  if (max_pages < 0 || tokens > INT_MAX) return fail(TQ_ERR_BAD_ARG, "tokens, batch and max_pages must be non-negative");
+  rc = check_heads(tokens, query_heads, kv_heads);
+  if (rc) return rc;
+  *p = plan_attention(tokens, batch, ragged != 0, query_heads / kv_heads, kv_heads, head_dim, max_pages, page_size, max_tokens,
+                      num_cus > 0 ? num_cus : device_cu_count());
+  return TQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t tq_paged_attention_workspace_bytes(int64_t tokens, int batch, int ragged, int query_heads, int kv_heads,
                                           int head_dim, int max_pages, int page_size, int64_t max_tokens, int num_cus) {
-  if (tokens <= 0 || batch <= 0 || kv_heads <= 0 || query_heads <= 0 || query_heads % kv_heads != 0 || max_pages < 0 ||
-      check_pages(1, page_size, kv_heads, head_dim) != TQ_OK)
+  PagedPlan p{};
+  if (tokens <= 0 || batch <= 0 ||
+      plan_for(tokens, batch, ragged, query_heads, kv_heads, head_dim, max_pages, page_size, max_tokens, num_cus, &p) != TQ_OK)
     return 0;
-  if (num_cus <= 0) num_cus = device_cu_count();
-  const PagedPlan p = plan_attention(tokens, batch, ragged != 0, query_heads / kv_heads, kv_heads, head_dim, max_pages, page_size, max_tokens, num_cus);
   return p.acc_bytes + p.ml_bytes + p.cut_bytes;
+}
+
+const char* tq_paged_attention_kernel(int64_t tokens, int batch, int ragged, int query_heads, int kv_heads, int head_dim,
+                                      int max_pages, int page_size, int64_t max_tokens, int num_cus) {
+  PagedPlan p{};
+  if (tokens <= 0 || batch <= 0) {
+    fail(TQ_ERR_BAD_ARG, "tokens and batch must be positive");
+    return nullptr;
+  }
+  if (plan_for(tokens, batch, ragged, query_heads, kv_heads, head_dim, max_pages, page_size, max_tokens, num_cus, &p) != TQ_OK) return nullptr;
+  const int d = head_dim == 64 ? 0 : head_dim == 128 ? 1 : 2;
+  static const char* const names[2][3] = {{"paged_split_kernel<64>", "paged_split_kernel<128>", "paged_split_kernel<256>"},
+                                          {"paged_chunk_kernel<64>", "paged_chunk_kernel<128>", "paged_chunk_kernel<256>"}};
+  return names[p.chunk ? 1 : 0][d];
 }
 
 int tq_paged_attention(const void* query, int64_t query_token_stride, int64_t query_head_stride, int query_dtype,

@@ -111,6 +111,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "tq_paged_dequantize": (_i, [_p, _i64, _p, _p, _p, _p, _i, _i, _i, _i, _p, _p, _i, _p]),
     "tq_paged_attention_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i, _i, _i, _i, _i64, _i]),
+    "tq_paged_attention_kernel": (ctypes.c_char_p, [_i64, _i, _i, _i, _i, _i, _i, _i, _i64, _i]),
     "tq_paged_attention": (
         _i,
         [_p, _i64, _i64, _i, _i64, _i, _i, _i, _p, _p, _p, _p, _i, _i, _p, _i64, _i, _p, _p, _i, _i64, _f, _p, _sz, _p,
@@ -164,7 +165,7 @@ def check(rc: int) -> None:
 
 
 _NOT_STATUS = {"tq_abi_version", "tq_last_error", "tq_decode_workspace_bytes", "tq_decode_split_kernel",
-               "tq_paged_attention_workspace_bytes"}
+               "tq_paged_attention_workspace_bytes", "tq_paged_attention_kernel"}
 
 
 def call(name: str, *args) -> int:
