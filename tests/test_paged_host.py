@@ -118,8 +118,8 @@ def test_workspace_bytes():
 def test_kernel_choice():
     name = lambda *a: _lib.call("tq_paged_attention_kernel", *a, 256)  # noqa: E731
     assert name(1, 1, 0, 32, 8, 128, 2000, 64, 1) == b"paged_split_kernel<128>"
-    assert name(16, 1, 1, 32, 8, 128, 500, 64, 16) == b"paged_chunk_kernel<128>"  # half a unit of rows over 32000 keys
-    assert name(15, 1, 1, 32, 8, 128, 500, 64, 15) == b"paged_split_kernel<128>"
+    assert name(16, 1, 1, 32, 8, 128, 512, 64, 16) == b"paged_chunk_kernel<128>"  # half a unit of rows over 32768 keys
+    assert name(15, 1, 1, 32, 8, 128, 9999, 64, 15) == b"paged_split_kernel<128>"
     assert name(128, 1, 1, 32, 8, 128, 32, 64, 128) == b"paged_split_kernel<128>"  # 512 rows over 2000 keys
     assert name(512, 1, 1, 32, 8, 128, 8, 64, 512) == b"paged_chunk_kernel<128>"  # enough units of rows
     assert name(64, 64, 1, 32, 8, 128, 500, 64, 0) == b"paged_split_kernel<128>"  # the most rows unknown: as if even
