@@ -78,38 +78,50 @@ __device__ __forceinline__ bool paged_angles(const PagedRotary& r, int l, int64_
     if ((r.axes_used >> k) & 1) good = good && row[k] >= 0 && row[k] < r.table_rows;
   }
   if (!good) return false;
+  if (PLAIN && r.axes > 1) {  // eight pairs: the rows of the axes among them, each taken where it is the pair's
+    uint32_t bits[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int d0 = h * (D / 2) + 8 * l, pair0 = d0 < half ? d0 : d0 - half;
+      uint32_t word = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) word = (pair0 >> 4) == k ? r.pair_axis[k] : word;
+      bits[h] = d0 < r.rotary_dim ? (word >> (2 * (pair0 & 8))) & 0xffffu : 0x10000u;  // bit 16: no pairs here
+    }
+#pragma unroll 1  // one axis's entries in registers at a time
+    for (int k = 0; k < r.axes; ++k) {
+      const int64_t at = k == 0 ? row[0] : k == 1 ? row[1] : k == 2 ? row[2] : row[3];
+      // pairs of axis k: two zero bits where the pair's axis and k agree
+      const uint32_t other = k * 0x5555u;
+      float ck[2][8], sk[2][8];
+      uint32_t same[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t x = (bits[h] & 0xffffu) ^ other;
+        same[h] = bits[h] >> 16 ? 0u : ~(x | (x >> 1)) & 0x5555u;
+        if (same[h] == 0) continue;
+        const int d0 = h * (D / 2) + 8 * l;
+        load8<TABLE>(r.cos, at * r.cos_stride + d0, r.table_type, true, ck[h]);
+        load8<TABLE>(r.sin, at * r.sin_stride + d0, r.table_type, true, sk[h]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool here = (same[h] >> (2 * i)) & 1;
+          c[8 * h + i] = here ? ck[h][i] : c[8 * h + i];
+          s[8 * h + i] = here ? sk[h][i] : s[8 * h + i];
+        }
+    }
+    return true;
+  }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int d0 = h * (D / 2) + 8 * l;
     if (d0 >= r.rotary_dim) continue;
-    if (r.axes == 1 && (PLAIN || d0 + 8 <= r.rotary_dim)) {
+    if (PLAIN || (r.axes == 1 && d0 + 8 <= r.rotary_dim)) {
       load8<TABLE>(r.cos, row[0] * r.cos_stride + d0, r.table_type, r.vec, c + 8 * h);
       load8<TABLE>(r.sin, row[0] * r.sin_stride + d0, r.table_type, r.vec, s + 8 * h);
-      continue;
-    }
-    if constexpr (PLAIN) {  // eight pairs: the rows of the axes among them, each taken where it is the pair's
-      const int pair0 = d0 < half ? d0 : d0 - half;
-      uint32_t bits = 0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) bits = (pair0 >> 4) == k ? r.pair_axis[k] : bits;
-      bits >>= 2 * (pair0 & 8);
-#pragma unroll 1  // one axis's entries in registers at a time
-      for (int k = 0; k < r.axes; ++k) {
-        const int64_t at = k == 0 ? row[0] : k == 1 ? row[1] : k == 2 ? row[2] : row[3];
-        bool has = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) has = has || ((bits >> (2 * i)) & 3) == k;
-        if (!has) continue;
-        float ck[8], sk[8];
-        load8<TABLE>(r.cos, at * r.cos_stride + d0, r.table_type, true, ck);
-        load8<TABLE>(r.sin, at * r.sin_stride + d0, r.table_type, true, sk);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const bool here = ((bits >> (2 * i)) & 3) == k;
-          c[8 * h + i] = here ? ck[i] : c[8 * h + i];
-          s[8 * h + i] = here ? sk[i] : s[8 * h + i];
-        }
-      }
       continue;
     }
 #pragma unroll
