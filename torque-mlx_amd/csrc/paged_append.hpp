@@ -198,17 +198,17 @@ __device__ __forceinline__ float over_root(float x) {
   return fabsf(q) < INFINITY ? y : q;
 }
 
-// This lane's signs before and after the transform, the second with the sign that
-// the transform's steps between lanes leave on it.
+// This lane's signs after the transform as bits (1: negative), with the sign that
+// the transform's steps between lanes leave.
 template <int D>
-__device__ __forceinline__ void basis_signs(const float* left, const float* right, int l, float (&first)[16], float (&second)[16]) {
+__device__ __forceinline__ uint32_t second_signs(const float* left, int l) {
+  uint32_t bits = 0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int d = (i >> 3) * (D / 2) + 8 * l + (i & 7);
-    first[i] = right[d];
-    second[i] = left[d];
-    if (__builtin_popcount(l) & 1) second[i] = -second[i];
-  }
+  for (int i = 0; i < 16; ++i) bits |= (__float_as_uint(left[(i >> 3) * (D / 2) + 8 * l + (i & 7)]) >> 31) << i;
+  return __builtin_popcount(l) & 1 ? ~bits : bits;
+}
+__device__ __forceinline__ float signed_by(float x, uint32_t bits, int i) {
+  return __uint_as_float(__float_as_uint(x) ^ ((bits << (31 - i)) & 0x80000000u));
 }
 
 // The Walsh-Hadamard transform of a row, in wave_fwht's order.
@@ -233,16 +233,6 @@ __device__ __forceinline__ void transform16(float (&v)[16], int l) {
     v[i] = __fadd_rn(x, y);
     v[i + 8] = __fsub_rn(x, y);
   }
-}
-
-// The rotated basis: wave_rotate's operations on the same operands.
-template <int D>
-__device__ __forceinline__ void into_basis(float (&v)[16], int l, const float (&first)[16], const float (&second)[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __fmul_rn(v[i], first[i]);
-  transform16<D>(v, l);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __fmul_rn(over_root<D>(v[i]), second[i]);
 }
 
 __device__ __forceinline__ int paged_code(float x, float inv) {
@@ -305,10 +295,12 @@ struct RowLoad<kAnyRows> {
 
 // What turns this lane's 16 elements of a token's rows, the same for all of its
 // heads: table entries, with the first signs in them (exactly: they are +-1), and
-// the second signs.
+// the second signs.  The rotated basis takes wave_rotate's operations on the same
+// operands, so its float32 result is the same.
 template <int D>
 struct RowTurn {
-  float c[16], s[16], second[16];
+  float c[16], s[16];
+  uint32_t second;
   bool turned, based;
 
   // Whether element i is turned (eight are alike where the rows' kind is known).
@@ -324,13 +316,13 @@ struct RowTurn {
     const bool good = !rotary || paged_angles<D, KIND>(a.rotary, l, token, position, c, s);
     turned = turned && good;
     if (based) {
-      float first[16];
-      basis_signs<D>(a.signs_left, a.signs_right, l, first, second);
+      second = second_signs<D>(a.signs_left, l);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
+        const float first = a.signs_right[(i >> 3) * (D / 2) + 8 * l + (i & 7)];
         const bool table = turned && in_table<KIND>(a, l, i);
-        c[i] = table ? c[i] * first[i] : first[i];
-        s[i] = table ? s[i] * first[i] : 0.f;
+        c[i] = table ? c[i] * first : first;
+        s[i] = table ? s[i] * first : 0.f;
       }
     }
     return good;
@@ -348,10 +340,10 @@ struct RowTurn {
     transform16<D>(v, l);
     if (rough) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = v[i] * kInverseRoot<D> * second[i];
+      for (int i = 0; i < 16; ++i) v[i] = signed_by(v[i] * kInverseRoot<D>, second, i);
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = __fmul_rn(over_root<D>(v[i]), second[i]);
+      for (int i = 0; i < 16; ++i) v[i] = signed_by(over_root<D>(v[i]), second, i);
     }
   }
 };
@@ -383,7 +375,7 @@ struct RowTurn {
 constexpr int append_threads(int d, int size) { return size == 0 ? kWave : d * size / 16; }
 
 template <int D, int SIZE, int KIND>
-__global__ __launch_bounds__(append_threads(D, SIZE)) __attribute__((amdgpu_waves_per_eu(KIND == kAnyRows ? 2 : 4)))
+__global__ __launch_bounds__(append_threads(D, SIZE)) __attribute__((amdgpu_waves_per_eu(KIND == kAnyRows ? 2 : KIND == kTypeF32 && append_threads(D, SIZE) <= 256 ? 3 : 4)))
 void paged_append_kernel(const PagedAppendArgs a) {
   constexpr int NT = append_threads(D, SIZE), WAVES = NT / kWave;
   constexpr int LPR = D / 16;  // lanes to a row
