@@ -99,8 +99,10 @@ int launch_planned(const PagedAttentionArgs& a, const PagedPlan& plan, hipStream
     hipLaunchKernelGGL((paged_merge_kernel<D, kChunkRows, 1>), merge, dim3(kBlock), 0, stream, a);
   else if (plan.workgroups < 8 * plan.items)  // fewer than 8 parts to a row, by and large
     hipLaunchKernelGGL((paged_merge_kernel<D, kSplitRows, 1>), merge, dim3(kBlock), 0, stream, a);
+  else if (plan.workgroups < 64 * plan.items)
+    hipLaunchKernelGGL((paged_merge_kernel<D, kSplitRows, 4>), dim3(static_cast<unsigned>(rows)), dim3(4 * kWave), 0, stream, a);
   else
-    hipLaunchKernelGGL((paged_merge_kernel<D, kSplitRows, kWavesPerBlock>), dim3(static_cast<unsigned>(rows)), dim3(kBlock), 0, stream, a);
+    hipLaunchKernelGGL((paged_merge_kernel<D, kSplitRows, 16>), dim3(static_cast<unsigned>(rows)), dim3(16 * kWave), 0, stream, a);
   return launch_status("paged_merge_kernel");
 }
 

@@ -300,28 +300,34 @@ __global__ __launch_bounds__(split_waves(D) * kWave, split_waves(D) / 4) void pa
       const int id = tile < to && t < it.s.len ? list[t >> p.log_page] : -1;
       return id < p.num_pages ? id : -1;  // below 0: none either
     };
-    PagedI4 kv[4][C], vv[DT];
-    float ks, vs;
-    auto load_keys = [&](int tile, int id) {
+    struct Tile {  // a tile's keys, values and scales, as this lane multiplies them
+      PagedI4 kv[4][C], vv[DT];
+      float ks, vs;
+    };
+    auto load_keys = [&](Tile& x, int tile, int id) {
       const int64_t page = static_cast<int64_t>(max(id, 0)) * p.kv_heads + h;
       const int first = (tile * kTile + 16 * (j >> 2)) & (T - 1);
       const int8_t* kp = a.key_pages + page * (D << p.log_page) + (first + (j & 3)) * D + 16 * g;
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int c = 0; c < C; ++c) kv[s][c] = *reinterpret_cast<const PagedI4*>(kp + 4 * s * D + 64 * c);
+        for (int c = 0; c < C; ++c) x.kv[s][c] = *reinterpret_cast<const PagedI4*>(kp + 4 * s * D + 64 * c);
     };
-    auto load_values = [&](int tile, int id) {
+    auto load_values = [&](Tile& x, int tile, int id) {
       const int64_t page = static_cast<int64_t>(max(id, 0)) * p.kv_heads + h;
       const int8_t* vp = a.value_pages + page * (D << p.log_page) + ((tile * kTile + 16 * g) & (T - 1)) + j * T;
 #pragma unroll
-      for (int t = 0; t < DT; ++t) vv[t] = *reinterpret_cast<const PagedI4*>(vp + 16 * t * T);
+      for (int t = 0; t < DT; ++t) x.vv[t] = *reinterpret_cast<const PagedI4*>(vp + 16 * t * T);
     };
-    auto load_scales = [&](int id) {
+    auto load_scales = [&](Tile& x, int id) {
       const int64_t page = static_cast<int64_t>(max(id, 0)) * p.kv_heads + h;
-      ks = a.key_scales[page];
-      vs = a.value_scales[page];
+      x.ks = a.key_scales[page];
+      x.vs = a.value_scales[page];
     };
+    // Two sets of registers at head_dim 256, whose wavefronts have 512 each and a SIMD to themselves: the next tile is
+    // on its way while one is multiplied.  Elsewhere one set, reloaded as its keys, then its values are done with.
+    constexpr bool kAhead = D == 256;
+    Tile tiles[kAhead ? 2 : 1];
     // The query row's load goes first: loads return in order, and its digits are made while keys are on their way.
     const bool live = j < it.rows;
     const PagedRowAt at = paged_row(a, it, h, live ? j : 0);
@@ -335,9 +341,9 @@ __global__ __launch_bounds__(split_waves(D) * kWave, split_waves(D) / 4) void pa
       const int kid = page_of(tile, j >> 2);
       knext = page_of(tile + kSplitWaves, j >> 2);
       vnext = page_of(tile + kSplitWaves, g);
-      load_keys(tile, kid);
-      load_scales(vid);
-      load_values(tile, vid);
+      load_keys(tiles[0], tile, kid);
+      load_scales(tiles[0], vid);
+      load_values(tiles[0], tile, vid);
     }
     // ---- this lane's query row, 16 dimensions of each chunk of 64
     PagedI4 q[PLANES][C];
@@ -366,10 +372,17 @@ __global__ __launch_bounds__(split_waves(D) * kWave, split_waves(D) / 4) void pa
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[t][r] = 0.f;
 
-    for (; tile < to; tile += kSplitWaves) {
+    auto step = [&](Tile& now, Tile& then) {
+      const auto& kv = now.kv;
+      const auto& vv = now.vv;
+      if (kAhead && tile + kSplitWaves < to) {
+        load_keys(then, tile + kSplitWaves, knext);
+        load_scales(then, vnext);
+        load_values(then, tile + kSplitWaves, vnext);
+      }
       const int64_t vt = static_cast<int64_t>(tile) * kTile + 16 * g;
       const int kafter = page_of(tile + 2 * kSplitWaves, j >> 2), vafter = page_of(tile + 2 * kSplitWaves, g);
-      const float by = ks * unit, shift = __log2f(vs), back = 1.f / vs;
+      const float by = now.ks * unit, shift = __log2f(now.vs), back = 1.f / now.vs;
       const int seen = vid >= 0 ? static_cast<int>(min(max(keys - vt, int64_t(0)), int64_t(16))) : 0;  // of its 16 tokens
 
       float w[16];
@@ -400,9 +413,9 @@ __global__ __launch_bounds__(split_waves(D) * kWave, split_waves(D) / 4) void pa
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, w[i]);
-      if (tile + kSplitWaves < to) {
-        load_keys(tile + kSplitWaves, knext);
-        load_scales(vnext);
+      if (!kAhead && tile + kSplitWaves < to) {
+        load_keys(then, tile + kSplitWaves, knext);
+        load_scales(then, vnext);
       }
       top = xor_reduce<32, OpMax>(xor_reduce<16, OpMax>(top));
       const float base = top == -INFINITY ? 0.f : top;
@@ -452,10 +465,16 @@ __global__ __launch_bounds__(split_waves(D) * kWave, split_waves(D) / 4) void pa
           acc[t][r] = fmaf(f, part, acc[t][r]);
         }
       }
-      if (tile + kSplitWaves < to) load_values(tile + kSplitWaves, vnext);
+      if (!kAhead && tile + kSplitWaves < to) load_values(then, tile + kSplitWaves, vnext);
       vid = vnext;
       knext = kafter;
       vnext = vafter;
+      tile += kSplitWaves;
+    };
+    while (tile < to) {
+      step(tiles[0], tiles[kAhead ? 1 : 0]);
+      if constexpr (kAhead)
+        if (tile < to) step(tiles[1], tiles[0]);
     }
 
     // ---- the wavefronts' sums as one
@@ -504,12 +523,13 @@ __global__ __launch_bounds__(split_waves(D) * kWave, split_waves(D) / 4) void pa
 }
 
 // Rows whose keys were cut: the parts' sums, brought to the largest maximum and
-// added in a fixed order.  WAVES wavefronts to a row: one, or four that take every
-// fourth part where rows are few and parts many.
+// added in a fixed order.  WAVES wavefronts to a row deal its parts out: one below
+// 8 parts, 4, and 16 from 64 parts on (128 parts of head_dim 256: 27 us with one
+// wavefront, 6.5 with 4, 5.9 with 16; 32 parts of 128: 8.6 with one, 3.9 with 4, 4.7 with 16).
 template <int D, int R, int WAVES>
-__global__ __launch_bounds__(kBlock) void paged_merge_kernel(const PagedAttentionArgs a) {
+__global__ __launch_bounds__(WAVES == 1 ? kBlock : WAVES * kWave) void paged_merge_kernel(const PagedAttentionArgs a) {
   constexpr int E = D / kWave;
-  __shared__ float s_sum[kWavesPerBlock][D + 2];
+  __shared__ float s_sum[WAVES][D + 2];
   const PagedBatch& p = a.batch;
   const int heads = p.kv_heads * a.group, wave = threadIdx.x >> 6, lane = lane_id();
   const uint32_t row = WAVES == 1 ? blockIdx.x * kWavesPerBlock + wave : blockIdx.x;
