@@ -366,6 +366,9 @@ struct RowTurn {
 // the bound at prompt sizes, the launch and three dependent loads (length, page
 // number, scale) at single tokens.
 //
+// 32768 tokens of 8 heads (and 32 query heads) of 128 in float16 take 175 us, 4.2
+// TB/s over the 738 MB read and written; one token of one sequence 5.3 us.
+//
 // KIND: the type of all rows, which are 16-byte aligned, as are float32 tables,
 // and rotary_dim a multiple of 16; or kAnyRows, which looks each of these up and
 // fetches elements one by one where it must, in twice the registers.

@@ -260,11 +260,10 @@ __device__ __forceinline__ float paged_unit(uint32_t top, float* f) {
 // from memory to the matrix instructions' operands.
 //
 // The codes are multiplied as they are, in v_mfma_i32_16x16x64_i8.  A query row
-// is an integer in PLANES balanced base-256 digits (|q| <= 127 x 256^(PLANES-1),
-// relative to the row's largest element): digits times codes sum exactly in 32
-// bits, so a score is as good as the query's rounding, 2^-16 of its largest
-// element with two digits (float16 and bfloat16 queries) and 2^-24 with three
-// (float32).  The weights of a tile, relative to the tile's own largest, are
+// is integers in PLANES balanced base-256 digits, relative to the row's largest
+// element: digits times codes sum exactly in 32 bits, so a score is as good as the
+// query's rounding, 2^-16 of its largest element with two digits (float16 and
+// bfloat16 queries) and 2^-23 with three (float32).  The weights of a tile, relative to the tile's own largest, are
 // held the same way; the sums over tokens are exact integers and enter the
 // running float32 sums once a tile.  A value page's scale vs goes into the
 // weight's exponent: w = exp2(s + log2 vs - max), and w / vs sums to the
@@ -275,6 +274,12 @@ __device__ __forceinline__ float paged_unit(uint32_t top, float* f) {
 // which is what it needs as the second product's right operand: 16 bytes of
 // weights for 16 bytes of values that lie side by side in the transposed page.
 //
+// Memory bounds it where a unit's 16 rows are few for the bytes of a key: 48 ragged
+// sequences of up to 8000 tokens (4 heads of 128, 189 MB) take 44.7 us, 4.2 TB/s,
+// 131072 tokens of 2 heads of 256 (float32 queries, 134 MB) 34 us.  A call of one
+// sequence first waits 4.5 us for the launch, its length, page numbers and first
+// keys (32768 tokens of 8 heads of 128: 16.8 us for 67 MB).  With 64 dimensions to
+// a score the vector instructions count more (about 280 a tile and wavefront).
 // A wavefront's next keys are on their way from the moment the current ones are
 // multiplied, its next values likewise, and page numbers a tile before that.
 constexpr int split_waves(int d) { return d == 256 ? 4 : d == 128 ? 8 : 12; }

@@ -155,6 +155,11 @@ struct DigitScores {
 // carry 2^7, so that they stay below float16's largest and a weight of 2^-31 of
 // the largest still counts.
 //
+// Measured: 2048 tokens of 32 query heads after 6000, head_dim 128, bfloat16: 369 us,
+// 638 TFLOP/s; 2000 tokens of 16 after 6001 at 256: 354 us, 646 TFLOP/s without the
+// merge, the matrix pipe 31 % busy: the wavefronts of a SIMD come to the exponentials
+// together, after the same barriers.
+//
 // Score register r of lane (column j, g = lane / 32) is the 32x32 product's row
 // 8 (r / 4) + 4 g + r mod 4; the key at that row is token 16 (r / 8) + 8 g +
 // r mod 8, so eight registers are the eight tokens of a 16-deep right operand
