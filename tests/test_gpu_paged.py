@@ -447,6 +447,62 @@ def test_append_bad_pages_and_lengths(hip_device):
     assert bool(((k - key[-2:].double().cpu()).abs() <= 0.5 * ks[..., None]).all())
 
 
+@pytest.mark.parametrize("dim,rotary", [(64, 64), (128, 40), (256, 128)])
+def test_append_types_and_strides_of_each_operand(hip_device, dim, rotary):
+    """float32 queries beside bfloat16 keys that lie unaligned in a larger tensor, expanded values, strided tables: as the
+    same rows laid out plainly."""
+    news, lens, kv = [37, 1, 20], [40, 1, 84], 2
+    n = sum(news)
+    wide = randn(1, n, 3, dim + 6, dtype=torch.bfloat16)
+    key = wide[:, :2, 3 : dim + 3]
+    value = randn(2, n, 1, dim, dtype=torch.bfloat16).expand(n, kv, dim)
+    query = randn(3, n, 4, 2 * dim)[..., 1::2]
+    cos, sin = (t[::2] for t in tables(200, rotary))
+    left, right = torch.sign(randn(8, dim)), torch.sign(randn(9, dim))
+    results = []
+    for k, v, q, c, s in ((key, value, query, cos, sin), tuple(t.contiguous() for t in (key, value, query, cos, sin))):
+        pool = model.Pool(lens, kv=kv, dim=dim, size=32, seed=3).fill()
+        out = ops.paged_append(k, v, query=q, cos=c, sin=s, signs_left=left, signs_right=right, rotate_values=True, page_table=pool.table,
+                               context_lens=pool.lens, token_starts=starts_of(news), **pool.t)
+        same = ops.paged_append(k, v, query=q.to(k.dtype), cos=c, sin=s, signs_left=left, signs_right=right, rotate_values=True,
+                                page_table=pool.table, context_lens=pool.lens, token_starts=starts_of(news), **pool.t)
+        results.append((out, same, *pool.t.values()))
+    assert results[0][0].dtype is torch.float32 and results[0][1].dtype is torch.bfloat16
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_attention_refuses_outputs_that_overlap(hip_device):
+    pool = model.Pool([30, 30], seed=1).fill()
+    query = randn(1, 2, 4, 64)
+    kw = dict(page_table=pool.table, context_lens=pool.lens, **pool.t)
+    for out, message in ((query, "share memory"), (torch.zeros(1, 4, 64, device="cuda").expand(2, 4, 64), "overlap itself"),
+                         (torch.zeros(2, 4, 64, dtype=torch.float16, device="cuda"), "out must be"),
+                         (torch.zeros(2, 4, 128, device="cuda")[..., ::2], "unit stride")):
+        with pytest.raises(ValueError, match=message):
+            ops.paged_attention(query, out=out, **kw)
+    with pytest.raises(ValueError, match="no backward"):
+        ops.paged_attention(query.clone().requires_grad_(), **kw)
+    with pytest.raises(ValueError, match="max_tokens"):
+        ops.paged_attention(query, max_tokens=0, **kw)
+
+
+def test_empty_calls(hip_device):
+    """No tokens, no sequences, a table without places."""
+    pool = model.Pool([5, 0], seed=1).fill()
+    none = torch.zeros(3, dtype=torch.int32, device="cuda")
+    x = torch.zeros(0, 2, 64, device="cuda")
+    before = {n: t.clone() for n, t in pool.t.items()}
+    kw = dict(page_table=pool.table, context_lens=pool.lens, token_starts=none, **pool.t)
+    assert ops.paged_append(x, x, query=x, **kw).shape == (0, 2, 64) and ops.paged_attention(x, **kw).shape == (0, 2, 64)
+    empty = dict(page_table=pool.table[:0], context_lens=pool.lens[:0], **pool.t)
+    assert ops.paged_append(x, x, **empty) is None and ops.paged_attention(x, **empty).shape == (0, 2, 64)
+    assert all(torch.equal(before[n], t) for n, t in pool.t.items())
+    bare = dict(page_table=pool.table[:, :0], context_lens=pool.lens, **pool.t)
+    assert bool((ops.paged_attention(randn(1, 2, 4, 64), **bare) == 0).all())
+    ops.paged_append(randn(1, 2, 2, 64), randn(2, 2, 2, 64), **bare)
+    assert all(torch.equal(before[n], t) for n, t in pool.t.items())
+
+
 def test_dequantize(hip_device):
     pool = model.Pool([200], kv=3, dim=128, size=32, seed=3).fill()
     ids = torch.tensor([3, 0, -1, pool.count, 3], dtype=torch.int32, device="cuda")

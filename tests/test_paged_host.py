@@ -93,6 +93,7 @@ def attention_args(**changes):
     (dict(ws=None), "workspace too small"),
     (dict(ws=FAKE + 4), "aligned"),
     (dict(tokens=2**30, starts=FAKE), "2\\^31"),
+    (dict(tokens=2**22, batch=2**22, table_stride=8, max_pages=8), "exceed one launch"),
 ])
 def test_attention_refusals(changes, message):
     with pytest.raises(ValueError, match=message):

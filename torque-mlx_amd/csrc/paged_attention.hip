@@ -29,6 +29,7 @@ struct PagedPlan {
 };
 
 constexpr int kSplitRows = 16;
+constexpr int64_t kMostUnits = int64_t(1) << 22;  // workgroups of up to 768 threads: a launch holds 2^32 - 1 work-items
 constexpr int kLeastTiles = 8;  // tiles of 64 keys that a workgroup takes at least
 
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -172,7 +173,8 @@ int tq_paged_attention(const void* query, int64_t query_token_stride, int64_t qu
   if (!aligned16(key_pages) || !aligned16(value_pages)) return fail(TQ_ERR_BAD_ARG, "pages must be 16-byte aligned");
   const int group = query_heads / kv_heads;
   const PagedPlan plan = plan_attention(tokens, batch, token_starts != nullptr, group, kv_heads, head_dim, max_pages, page_size, max_tokens, device_cu_count());
-  if (plan.items > INT_MAX) return fail(TQ_ERR_BAD_ARG, "tokens x group exceeds one launch");
+  if (plan.items > INT_MAX || (plan.workgroups == 0 && plan.items * kv_heads > kMostUnits))
+    return fail(TQ_ERR_BAD_ARG, "tokens x heads exceed one launch; attend with fewer sequences per call");
   const size_t need = plan.acc_bytes + plan.ml_bytes + plan.cut_bytes;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(TQ_ERR_BAD_ARG, "workspace too small: " + std::to_string(workspace_bytes) + " bytes, the call needs " + std::to_string(need));

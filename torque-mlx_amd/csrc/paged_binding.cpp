@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
@@ -266,6 +267,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK_VALUE(!(out.requires_grad() && at::GradMode::is_enabled()),
                       "the paged cache has no backward pass: out wants a gradient (use torch.no_grad())");
     TORCH_CHECK_VALUE(!out.storage().is_alias_of(query.storage()), "out must not share memory with query");
+    TORCH_CHECK_VALUE(at::has_internal_overlap(out) != at::MemOverlap::Yes, "out must not overlap itself");
   }
   const size_t bytes = g_workspace(tokens, batch.batch, batch.starts != nullptr, static_cast<int>(heads), pool.heads, pool.dim, batch.width,
                                    pool.size, most, 0);

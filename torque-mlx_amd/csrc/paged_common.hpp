@@ -40,6 +40,9 @@ struct PagedBatch {
   int kv_heads;
 };
 
+// Tokens of a sequence, at most: a tile's last token is counted in 32 bits too.
+constexpr int64_t kMostTokens = 0x7fffff00;
+
 struct PagedSequence {
   int row0, rows;  // its rows of the call
   int len;         // its tokens, at most what the page table holds and at least 0
@@ -61,7 +64,7 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch& p, int
   }
   const int64_t len = p.lens[b];
   s.first = len - s.rows;
-  s.len = static_cast<int>(min(max(len, int64_t(0)), static_cast<int64_t>(p.max_pages) << p.log_page));
+  s.len = static_cast<int>(min(min(max(len, int64_t(0)), kMostTokens), static_cast<int64_t>(p.max_pages) << p.log_page));
   return s;
 }
 

@@ -134,8 +134,10 @@ class TorquePagedKVCache:
                 self._table[s, first : first + more] = torch.tensor(self._pages[s][first:], dtype=torch.int32, device=self.device)
 
     def _batch(self, seqs: list[int], counts: list[int]) -> dict[str, Any]:
-        table = self._table[: len(seqs)] if seqs == list(range(len(seqs))) else self._table[torch.tensor(seqs, device=self.device)]
         numbers = [self._lengths[s] for s in seqs]
+        # no wider than the longest sequence: the width is what the attention's choice of kernel knows of the lengths
+        table = self._table[:, : max(1, -(-max(numbers, default=0) // self.page_size))]
+        table = table[: len(seqs)] if seqs == list(range(len(seqs))) else table[torch.tensor(seqs, device=self.device)]
         if counts == [1] * len(seqs):
             return dict(page_table=table, context_lens=torch.tensor(numbers, dtype=torch.int32, device=self.device), token_starts=None)
         starts = [0]

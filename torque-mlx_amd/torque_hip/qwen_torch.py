@@ -250,7 +250,7 @@ class QwenTorquePagedCacheHIP:
         q, k, v = (x.transpose(1, 2).reshape(batch * length, x.shape[1], x.shape[3]) for x in (queries, keys, values))
         tables: dict[str, Any] = {}
         if cos is not None and sin is not None:
-            flat = [t.expand(batch, -1, -1).reshape(batch * length, t.shape[-1]) for t in (cos, sin)]
+            flat = [t.float().expand(batch, -1, -1).reshape(batch * length, t.shape[-1]) for t in (cos, sin)]
             tables = dict(cos=flat[0], sin=flat[1], tables_by_token=True)
         counts = [length] * batch
         q = self.paged.append(k, v, query=q, sequences=self.sequences, counts=counts, **tables)
