@@ -65,6 +65,20 @@ def test_attention_against_64_bits(hip_device, dim, size, dtype, kv, group, news
         check_attention(pool, query, news, lens, same)
 
 
+@pytest.mark.parametrize("dim,size,dtype,kv,group,news,lens", [c for c in ATTENTION if max(c[5]) * c[4] < 64])
+def test_cut_keys_against_64_bits(hip_device, dim, size, dtype, kv, group, news, lens):
+    """A table wide enough for long sequences has the keys cut over workgroups, whatever the lengths are."""
+    pool = model.Pool(lens, kv=kv, dim=dim, size=size, seed=3, width=20_000 // size).fill()
+    query = randn(5, sum(news), kv * group, dim, dtype=TYPES[dtype])
+    ragged = news != [1] * len(lens)
+    shape = (sum(news), len(lens), int(ragged), kv * group, kv, dim, pool.table.shape[1], size, max(news), 0)
+    assert _lib.call("tq_paged_attention_workspace_bytes", *shape) > 0
+    kw = dict(page_table=pool.table, context_lens=pool.lens, token_starts=starts_of(news) if ragged else None, max_tokens=max(news))
+    out = ops.paged_attention(query, **kw, **pool.t)
+    check_attention(pool, query, news, lens, out)
+    assert torch.equal(out, ops.paged_attention(query, **kw, **pool.t))
+
+
 CHUNKS = [
     # dim, page, dtype, kv, group, tokens each sequence adds, lengths with them
     (128, 64, "bf16", 1, 4, [70, 0, 33], [70, 10, 300]),
@@ -220,7 +234,7 @@ def test_scale_and_bad_queries(hip_device):
 
 
 @pytest.mark.parametrize("spread", [0, 30])
-@pytest.mark.parametrize("new,width", [(1, 32), (100, 32), (100, 4096)])
+@pytest.mark.parametrize("new,width", [(1, 32), (1, 4096), (100, 32), (100, 4096)])
 def test_scales_far_apart(hip_device, spread, new, width):
     """Pages whose scales differ by up to 2^30, one sharp row among them."""
     lens = [500]
@@ -552,14 +566,15 @@ def graph_step(pool, dtype, kv, group, dim, tokens, starts):
     return bufs, step
 
 
+@pytest.mark.parametrize("width", [None, 100])  # of the table: keys read by one workgroup, and cut with a workspace
 @pytest.mark.parametrize("news", [[1, 1], [40, 7]])
-def test_graphs_follow_the_lengths(hip_device, news):
+def test_graphs_follow_the_lengths(hip_device, news, width):
     """Two captured steps replayed in turn, other lengths and rows each time, eager work between: each as the eager step."""
     kv, group, dim = 2, 2, 128
     most = 700
     pools, graphs = [], []
     for i in range(2):
-        pool = model.Pool([most, most], kv=kv, dim=dim, size=32, seed=i)
+        pool = model.Pool([most, most], kv=kv, dim=dim, size=32, seed=i, width=width)
         bufs, step = graph_step(pool, torch.float16, kv, group, dim, sum(news), None if news == [1, 1] else starts_of(news))
         pool.lens.copy_(torch.tensor(news, dtype=torch.int32))
         side = torch.cuda.Stream()

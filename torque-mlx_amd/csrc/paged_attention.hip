@@ -51,6 +51,12 @@ constexpr int64_t kChunkRowsLeast = kChunkRows / 2;
 constexpr int64_t kChunkUnits = 128;
 constexpr double kChunkWork = 1 << 18;
 
+// The most tiles of a sequence that one workgroup walks alone, with no merge: two for
+// each wavefront of the split kernel.  Uncut / cut in us, 16-bit queries: 8 sequences of
+// 1000 tokens 7.8 / 12.1 at head_dim 64, 11.7 / 14.2 at 128; of 1500 tokens 9.2 / 12.3 and
+// 14.2 / 14.7; at head_dim 256 600 tokens 18.5 / 26.7 and 1000 already 23.7 / 20.5.
+int whole_tiles(bool chunk, int head_dim) { return chunk ? kLeastTiles : 2 * split_waves(head_dim); }
+
 PagedPlan plan_attention(int64_t tokens, int batch, bool ragged, int group, int kv_heads, int head_dim, int max_pages,
                          int page_size, int64_t max_tokens, int num_cus) {
   PagedPlan p{};
@@ -63,7 +69,7 @@ PagedPlan plan_attention(int64_t tokens, int batch, bool ragged, int group, int 
   p.rows = p.chunk ? kChunkRows : kSplitRows;
   p.items = ragged ? tokens * group / p.rows + batch : static_cast<int64_t>(batch) * ((group + p.rows - 1) / p.rows);
   const int64_t units = p.items * kv_heads;
-  if (tiles <= kLeastTiles || units >= (p.chunk ? 1 : 16) * static_cast<int64_t>(num_cus) || p.items * tiles >= INT_MAX) return p;
+  if (tiles <= whole_tiles(p.chunk, head_dim) || units >= (p.chunk ? 1 : 16) * static_cast<int64_t>(num_cus) || p.items * tiles >= INT_MAX) return p;
   const int64_t fill = std::max<int64_t>(1, (p.chunk ? (head_dim == 256 ? 1 : 2) : 1) * static_cast<int64_t>(num_cus) / kv_heads);
   const int64_t most = std::max<int64_t>(1, (p.items * tiles + kLeastTiles - 1) / kLeastTiles);
   p.workgroups = static_cast<int>(std::min(fill, most));
