@@ -19,11 +19,16 @@ using namespace tq;
 
 namespace {
 
-// Heads to a workgroup of an append, which share their tokens' table entries: as
-// many (8 at most) as leave this many workgroups.
-constexpr int64_t kAppendBlocks = 1024;
-int heads_to_block(int64_t rows, int heads) {
-  return static_cast<int>(std::min<int64_t>(8, std::max<int64_t>(1, rows * heads / kAppendBlocks)));
+// Heads to a workgroup of an append, which share their tokens' table entries and
+// fetch one head's rows while another's are worked on: as many (8 at most) as leave
+// this many threads, half of what the GPU holds at once at 128 registers.  8192 tokens
+// (1024 elements of the cache to each, bfloat16) in us with 2^17 / 2^18 / 2^19 / 2^20 and
+// with 1024 workgroups of whatever size: head_dim 256, pages of 64 54 / 53 / 64 / 85 / 85,
+// pages of 16 45 / 45 / 49 / 64 / 45; 128, pages of 64 42 / 46 / 53 / 61 / 53; 64, pages of
+// 16 39 / 41 / 42 / 48 / 39.
+constexpr int64_t kAppendThreads = int64_t(1) << 17;
+int heads_to_block(int64_t rows, int heads, int threads) {
+  return static_cast<int>(std::min<int64_t>(8, std::max<int64_t>(1, rows * heads * threads / kAppendThreads)));
 }
 
 template <int D, int SIZE>
@@ -31,7 +36,7 @@ int launch_append(PagedAppendArgs a, hipStream_t stream) {
   constexpr int kThreads = append_threads(D, SIZE), kRows = kThreads / (D / 16);
   const int64_t batch = a.batch.batch, tokens = a.batch.tokens;
   const int64_t units = SIZE == 0 ? batch : (tokens >> a.batch.log_page) + 2 * batch;
-  a.kv_step = heads_to_block(2 * units, a.batch.kv_heads);
+  a.kv_step = heads_to_block(2 * units, a.batch.kv_heads, kThreads);
   a.kv_parts = (a.batch.kv_heads + a.kv_step - 1) / a.kv_step;
   a.kv_blocks = units * a.kv_parts * 2;
   int64_t blocks = a.kv_blocks;
@@ -39,7 +44,7 @@ int launch_append(PagedAppendArgs a, hipStream_t stream) {
                      (a.rotary.rotary_dim == 0 || (a.rotary.vec && a.rotary.table_type == TQ_F32 && a.rotary.rotary_dim % 16 == 0));
   if (a.query.data != nullptr) {
     const int64_t rows = (tokens + kRows - 1) / kRows;
-    a.query_step = heads_to_block(rows, a.query_heads);
+    a.query_step = heads_to_block(rows, a.query_heads, kThreads);
     a.query_parts = (a.query_heads + a.query_step - 1) / a.query_step;
     blocks += rows * a.query_parts;
   }
