@@ -111,8 +111,9 @@ def test_dequantize_refusals():
 
 def test_workspace_bytes():
     ws = lambda *a: int(_lib.call("tq_paged_attention_workspace_bytes", *a, 256))  # noqa: E731
-    for dim, pages in ((64, 24), (128, 16), (256, 8)):  # two tiles of 64 keys to a wavefront: nothing to join
-        assert ws(1, 1, 0, 8, 8, dim, pages, 64, 1) == 0 and ws(1, 1, 0, 8, 8, dim, pages + 1, 64, 1) > 0
+    for dim, few, many in ((64, 48, 64), (128, 24, 32), (256, 12, 16)):  # as many tiles of 64 keys, and nothing to join
+        assert ws(1, 1, 0, 8, 8, dim, few, 64, 1) == 0 and ws(1, 1, 0, 8, 8, dim, few + 1, 64, 1) > 0
+        assert ws(32, 32, 0, 8, 8, dim, many, 64, 1) == 0 and ws(32, 32, 0, 8, 8, dim, many + 1, 64, 1) > 0
     assert ws(1, 1, 0, 32, 8, 128, 512, 64, 1) > 0
     assert ws(1, 1, 0, 30, 8, 128, 512, 64, 1) == 0 and ws(1, 1, 0, 8, 8, 100, 512, 64, 1) == 0  # refused shapes
 

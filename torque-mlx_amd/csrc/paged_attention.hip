@@ -51,11 +51,20 @@ constexpr int64_t kChunkRowsLeast = kChunkRows / 2;
 constexpr int64_t kChunkUnits = 128;
 constexpr double kChunkWork = 1 << 18;
 
-// The most tiles of a sequence that one workgroup walks alone, with no merge: two for
-// each wavefront of the split kernel.  Uncut / cut in us, 16-bit queries: 8 sequences of
-// 1000 tokens 7.8 / 12.1 at head_dim 64, 11.7 / 14.2 at 128; of 1500 tokens 9.2 / 12.3 and
-// 14.2 / 14.7; at head_dim 256 600 tokens 18.5 / 26.7 and 1000 already 23.7 / 20.5.
-int whole_tiles(bool chunk, int head_dim) { return chunk ? kLeastTiles : 2 * split_waves(head_dim); }
+// The most tiles of a sequence that one workgroup walks alone, with no merge.  A tile
+// takes a workgroup of the split kernel 0.16, 0.34 and 1.04 us at head_dim 64, 128 and
+// 256, and cutting costs 4 to 8.  Uncut / cut in us, 16-bit queries, 8 heads (4 at 256):
+//   head_dim 64: one sequence of 1500 tokens 9.0 / 11.9, of 4000 15.5 / 11.7; eight of
+//   1500 9.2 / 12.3, of 4000 15.8 / 17.2
+//   head_dim 128: one of 1500 13.7 / 14.0, of 2000 16.3 / 14.7; eight of 1500 14.2 / 14.7,
+//   of 2000 16.6 / 15.6
+//   head_dim 256: eight of 600 18.5 / 26.7, of 1000 23.7 / 20.5
+// and where the sequences are enough for the GPU, some longer ones: of up to 2000 tokens
+// each, 32 at head_dim 64 11.3 / 23.6, at 128 19.3 / 31.2, 64 33.7 / 39.7, 256 129 / 125; of
+// up to 8000, 64 at 128 110 / 97, 128 at 256 306 / 204.
+int64_t whole_tiles(bool chunk, int64_t units, int num_cus, int head_dim) {
+  return chunk ? kLeastTiles : (units >= num_cus ? 64 : 48) * 64 / head_dim;
+}
 
 PagedPlan plan_attention(int64_t tokens, int batch, bool ragged, int group, int kv_heads, int head_dim, int max_pages,
                          int page_size, int64_t max_tokens, int num_cus) {
@@ -69,7 +78,7 @@ PagedPlan plan_attention(int64_t tokens, int batch, bool ragged, int group, int 
   p.rows = p.chunk ? kChunkRows : kSplitRows;
   p.items = ragged ? tokens * group / p.rows + batch : static_cast<int64_t>(batch) * ((group + p.rows - 1) / p.rows);
   const int64_t units = p.items * kv_heads;
-  if (tiles <= whole_tiles(p.chunk, head_dim) || units >= (p.chunk ? 1 : 16) * static_cast<int64_t>(num_cus) || p.items * tiles >= INT_MAX) return p;
+  if (tiles <= whole_tiles(p.chunk, units, num_cus, head_dim) || units >= (p.chunk ? 1 : 16) * static_cast<int64_t>(num_cus) || p.items * tiles >= INT_MAX) return p;
   const int64_t fill = std::max<int64_t>(1, (p.chunk ? (head_dim == 256 ? 1 : 2) : 1) * static_cast<int64_t>(num_cus) / kv_heads);
   const int64_t most = std::max<int64_t>(1, (p.items * tiles + kLeastTiles - 1) / kLeastTiles);
   p.workgroups = static_cast<int>(std::min(fill, most));
