@@ -288,7 +288,7 @@ template <int D, int PLANES, bool CUT>
 __global__ __launch_bounds__(split_waves(D) * kWave, split_waves(D) / 4) void paged_split_kernel(const PagedAttentionArgs a) {
   constexpr int R = 16, C = D / 64, DT = D / 16, kSplitWaves = split_waves(D);
   constexpr int P = D + 4;  // LDS pitch of a row of sums
-  constexpr float kUnit = PLANES == 3 ? 8323072.f : 32512.f;  // 127 x 256^(PLANES-1)
+  constexpr float kUnit = 127.f * (PLANES == 3 ? 65536.f : 256.f);  // 127 x 256^(PLANES-1)
   __shared__ __align__(16) float s_acc[kSplitWaves][R][P];
   __shared__ float s_ml[kSplitWaves][R][2];
   const PagedBatch& p = a.batch;
